@@ -35,6 +35,7 @@ extern "C" {
 #define PCFGNAT_F16 0
 #define PCFGNAT_F32 1
 #define PCFGNAT_F64 2
+#define PCFGNAT_BF16 3 /* the operators at the end of this header only */
 
 /* ABI version of this header (bumped on incompatible change). */
 int pcfgnat_abi_version(void);
@@ -430,6 +431,59 @@ int pcfgnat_viterbi_decoding_host(const int64_t *pred_length, const int64_t *out
                                   const int64_t *R, const int64_t *M, const int64_t *tokens,
                                   const int64_t *left_tree_mask, int64_t mask_dim, int64_t pad_index,
                                   int64_t *out_tokens, int64_t *out_count, int64_t B, int64_t L, int64_t Lq);
+
+/*
+ * Log-probabilities of given tokens over rows of logits, with the entropy of each row and its top alternatives: one read of
+ * the logits (no counterpart in the reference, whose model takes log_softmax and max,
+ * glat_decomposed_with_link_two_hands_tri_pcfg.py:414-415; pcfgnat_logsoftmax_max is that).
+ *   logits       outer x inner rows of V elements, F16 / BF16 / F32; row (b, p) starts at element
+ *                b * stride_outer + p * stride_inner, its elements are adjacent.  Any alignment of a whole element.
+ *   tokens       int64 [outer, inner] contiguous, or NULL: log-probabilities are not asked for.
+ *   logprobs     float32 [outer, inner]; NULL if and only if tokens is.
+ *   entropy      float32 [outer, inner], or NULL.
+ *   top          0..64 alternatives, at most V; top_logprobs float32 and top_tokens int64 [outer, inner, top], descending,
+ *                equal logits in ascending index (NaN counts as largest).
+ *   stats        float32 [3, outer * inner] (row maximum, log of the sum, entropy) for the backward, or NULL.
+ *   workspace    pcfgnat_token_logprobs_workspace_bytes bytes, 8-byte aligned; may be NULL where that is 0.
+ * A negative token leaves its row out: the row is not read, its outputs are 0, 0, -inf and -1.  A token at or beyond V has
+ * log-probability NaN.  A row of nothing but -inf has log-probabilities -inf and entropy 0; a NaN or +inf among the logits
+ * makes the row's log-probabilities and entropy NaN.
+ */
+size_t pcfgnat_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t V, int top);
+int pcfgnat_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer,
+                           int64_t stride_inner, const int64_t *tokens, float *logprobs, float *entropy, int top,
+                           float *top_logprobs, int64_t *top_tokens, float *stats, void *workspace, int64_t V, void *stream);
+
+/*
+ * Its backward: grad_logits [outer, inner, V] contiguous, in the logits' type,
+ *   grad[v] = sum_j g_j [v = id_j] - p_v (sum_j g_j + g_entropy (log p_v + H)),  j over the token and the alternatives,
+ * in float32, rounded once.  Any of grad_logprobs [rows], grad_entropy [rows], grad_top [rows, top] (float32, contiguous) may
+ * be NULL: nothing arrives there.  stats and top_tokens as the forward left them.  Rows left out and rows of nothing but
+ * -inf have gradient 0.  grad_logits must not overlap the logits.
+ */
+int pcfgnat_token_logprobs_backward(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer,
+                                    int64_t stride_inner, const int64_t *tokens, const int64_t *top_tokens, int top,
+                                    const float *stats, const float *grad_logprobs, const float *grad_entropy,
+                                    const float *grad_top, void *grad_logits, int64_t V, void *stream);
+
+/*
+ * Embedding lookup with scaling: out[n] = scale * weight[tokens[n]], rounded once (what the decoder does with the glanced
+ * tokens of nat_pcfg_loss.py:268 next).  weight [V, D], F16 / BF16 / F32, rows weight_stride elements apart; tokens int64
+ * [N]; out [N, D] contiguous.  A negative token is a row of zeros, one at or beyond V a row of NaN.
+ */
+int pcfgnat_token_embedding(const void *weight, int dtype, int64_t weight_stride, const int64_t *tokens, float scale,
+                            void *out, int64_t N, int64_t V, int64_t D, void *stream);
+
+/*
+ * Its gradient: grad_weight[v] = scale * sum of grad_out[n] over the n with tokens[n] = v, in float32 in an order that
+ * depends on the tokens alone (the same inputs give the same bits), rounded once; every row of grad_weight [V, D] (contiguous)
+ * is written.  grad_out rows are grad_stride elements apart.  padding_idx (negative: none) and tokens outside [0, V) have no
+ * gradient.  workspace: pcfgnat_token_embedding_backward_workspace_bytes bytes, 16-byte aligned.
+ */
+size_t pcfgnat_token_embedding_backward_workspace_bytes(int64_t N, int64_t V, int64_t D);
+int pcfgnat_token_embedding_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, float scale,
+                                     int64_t padding_idx, void *grad_weight, void *workspace, int64_t N, int64_t V, int64_t D,
+                                     void *stream);
 
 #ifdef __cplusplus
 }

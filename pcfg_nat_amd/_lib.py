@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libpcfg_nat_hip.so")
 EXT_PATH = os.path.join(_HERE, "lib", "_pcfg_nat_torch.so")
 
 OK, EINVAL, EUNSUPPORTED, EHIP = 0, 1, 2, 3
-F16, F32, F64 = 0, 1, 2
+F16, F32, F64, BF16 = 0, 1, 2, 3
 
 _lib = None
 _ext = None
@@ -80,6 +80,12 @@ SIGNATURES = {
     "pcfgnat_viterbi_decode_logits": (_int, [_vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "pcfgnat_lookahead_decode": (_int, [_vp, _vp, ctypes.c_float, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "pcfgnat_viterbi_decoding_host": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64]),
+    "pcfgnat_token_logprobs_workspace_bytes": (ctypes.c_size_t, [_int, _i64, _i64, _int]),
+    "pcfgnat_token_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "pcfgnat_token_logprobs_backward": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "pcfgnat_token_embedding": (_int, [_vp, _int, _i64, _vp, ctypes.c_float, _vp, _i64, _i64, _i64, _vp]),
+    "pcfgnat_token_embedding_backward_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "pcfgnat_token_embedding_backward": (_int, [_vp, _int, _i64, _vp, ctypes.c_float, _i64, _vp, _vp, _i64, _i64, _i64, _vp]),
 }
 
 

@@ -8,18 +8,12 @@
 //
 // Why it exists: a training step through the Python Functions costs the host about 0.25 ms (Function.apply, half a dozen
 // torch.empty, ctypes marshalling of twenty arguments, twice), more than the 0.17 ms its kernels run.
-#include <torch/extension.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-
-#include "../../include/pcfg_nat_hip.h"
+#include "torch_ext.h"
 
 namespace {
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-void check_rc(int rc) { TORCH_CHECK(rc == PCFGNAT_OK, pcfgnat_last_error()); }
 
 int dtype_code(const at::Tensor &t, const char *who) {
     switch (t.scalar_type()) {
@@ -27,18 +21,6 @@ int dtype_code(const at::Tensor &t, const char *who) {
         case at::kFloat: return PCFGNAT_F32;
         case at::kDouble: return PCFGNAT_F64;
         default: TORCH_CHECK(false, who, ": unsupported dtype ", t.scalar_type(), " (float16, float32, float64 are dispatched)");
-    }
-}
-
-void *stream_of(const at::Tensor &t) { return (void *)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-
-void need_gpu(const char *who, std::initializer_list<const at::Tensor *> ts) {
-    const at::Tensor *first = nullptr;
-    for (const at::Tensor *t : ts) {
-        if (t == nullptr || !t->defined()) continue;
-        TORCH_CHECK(t->is_cuda(), who, ": expected tensors on the GPU, got a ", t->device().type(), " tensor");
-        if (first == nullptr) first = t;
-        TORCH_CHECK(t->device() == first->device(), who, ": tensors are on different devices (", first->device(), " vs ", t->device(), ")");
     }
 }
 
@@ -475,4 +457,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "checks, allocation and enqueue of the single-call Viterbi decode (glat_decomposed_with_link_two_hands_tri_pcfg.py:414-416, 483-502)");
     m.def("pcfg_extract_links_fused", &pcfg_extract_links_fused,
           "the link scorer after its projections, products inside the kernels (glat_decomposed_with_link_two_hands_tri_pcfg.py:153-199)");
+    register_vocab_ops(m);
 }

@@ -12,6 +12,7 @@ import contextlib
 import ctypes
 import threading
 import time
+from typing import NamedTuple, Optional
 
 import torch
 from torch.autograd import Function
@@ -1318,3 +1319,40 @@ def pcfg_criterion(outputs, targets, links, output_length, target_length, matchm
     _, loss, ll, invalid = PCFGCriterionFunc.apply(outputs, links, targets, output_length, target_length, matchmask, keep_word_mask)
     return loss, ll, invalid
 
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` returns; ``None`` for what was not asked for."""
+    logprobs: Optional[torch.Tensor]      # [...] float32
+    entropy: Optional[torch.Tensor]       # [...] float32
+    top_logprobs: Optional[torch.Tensor]  # [..., top] float32, descending
+    top_tokens: Optional[torch.Tensor]    # [..., top] int64
+
+
+def token_logprobs(logits, tokens=None, top=0, entropy=False):
+    """Log-probabilities of given tokens under rows of vocabulary logits, with the entropy of each row's distribution and
+    its ``top`` most probable alternatives (0..64), from one read of the logits.  Beside ``logsoftmax_max``, which is the
+    model's own front-end (glat_decomposed_with_link_two_hands_tri_pcfg.py:414-415): any number of alternatives, given
+    tokens, bfloat16, strides, and a gradient.
+
+    ``logits`` [..., vocab] float16, bfloat16 or float32; ``tokens`` [...] int64, or None.  Up to two strides over the rows
+    are read in place (a slice of a padded vocabulary, a batch without its first node); other layouts are copied first.
+    Differentiable in the logits through all three results (once: ``create_graph`` raises); the gradient is computed in
+    float32 and rounded to the logits' type once.
+
+    * A negative token leaves its row out: it is not read; log-probability and entropy 0, alternatives -inf and -1,
+      gradient 0.  A token at or beyond the vocabulary has log-probability NaN.
+    * Equal logits are listed in ascending index; NaN counts as the largest value.
+    * -inf masks an entry.  A row of nothing but -inf has log-probabilities -inf, entropy 0 and gradient 0.  A NaN or +inf
+      makes the log-probabilities and the entropy of its row NaN."""
+    return TokenLogprobs(*_lib.load_ext().token_logprobs(logits, tokens, top, entropy))
+
+
+def token_embedding(weight, tokens, scale=1.0, padding_idx=None):
+    """``scale * weight[tokens]``, rounded to the weight's type once: what the decoder does with the tokens that
+    ``pcfg_glat_step`` leaves (``glat_prev_output_tokens``, nat_pcfg_loss.py:268).  ``weight`` [vocab, dim] float16, bfloat16
+    or float32 (rows any distance apart), ``tokens`` int64 of any shape; returns [*tokens.shape, dim].
+
+    Differentiable in the weight (once: ``create_graph`` raises): each row of the gradient is summed in float32, in an order
+    that depends on the tokens alone, and rounded once, so the same inputs give the same bits.  ``padding_idx``'s row has no
+    gradient.  A negative token is a row of zeros and one at or beyond the vocabulary a row of NaN, both without gradient."""
+    return _lib.load_ext().token_embedding(weight, tokens, scale, padding_idx)
