@@ -14,6 +14,7 @@ namespace pcfgnat {
 namespace {
 
 constexpr int MAX_TOP = 64;
+constexpr int64_t MAX_LOGPROB_VOCAB = (int64_t)64 * 512 * 10 * 4;  // MAX_PARTS parts of what a workgroup holds, of float32
 
 struct LogprobArgs {
     const int64_t *tokens;
@@ -23,6 +24,10 @@ struct LogprobArgs {
     int64_t rows, inner, so, si;
     int V, top;
 };
+
+// Makes the compiler forget what it knows about a chunk in registers, so that each pass widens it anew instead of keeping
+// the wide values alive.
+__device__ __forceinline__ void opaque(vec16 &v) { asm volatile("" : "+v"(v)); }
 
 // Order of the alternatives as a whole number: value first (NaN largest, -0 = +0), then the lower index.  Never 0
 // and never all ones, so both can stand for "no key".
@@ -48,85 +53,452 @@ __device__ __forceinline__ unsigned long long wave_max_key(unsigned long long v)
     return v;
 }
 
+// Row r of the logits.  (rows < 2^31: a 32-bit division, and none at all where one stride covers the rows)
 template <typename T>
-__device__ __forceinline__ const T *row_at(const T *logits, const LogprobArgs &a, int64_t r) {
-    const int64_t b = r / a.inner;
-    return logits + b * a.so + (r - b * a.inner) * a.si;
+__device__ __forceinline__ const T *row_at(const T *logits, unsigned r, int64_t inner, int64_t so, int64_t si, bool one_stride) {
+    if (one_stride) return logits + (int64_t)r * si;
+    const unsigned b = r / (unsigned)inner;
+    return logits + (int64_t)b * so + (int64_t)(r - b * (unsigned)inner) * si;
 }
 
+// Splits n elements at any element address into [head scalars][16-byte chunks][tail scalars].
 template <typename T>
-__global__ __launch_bounds__(256) void logprobs_kernel(const T *__restrict__ logits, LogprobArgs a) {
-    __shared__ float s_f[8];
-    __shared__ unsigned long long s_k[4];
-    const int64_t r = blockIdx.x;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int64_t tok = a.tokens ? a.tokens[r] : 0;
-    if (tok < 0) {
-        if (tid == 0) {
-            a.logprobs[r] = 0.f;
-            if (a.entropy) a.entropy[r] = 0.f;
-        }
-        if (tid < a.top) {
-            a.top_logprobs[r * a.top + tid] = NEG_INF_F;
-            a.top_tokens[r * a.top + tid] = -1;
-        }
-        return;
+struct Span {
+    int head, nvec, tail;
+    __device__ __forceinline__ Span(const T *x, int n) {
+        constexpr int N = VocabElem<T>::N;
+        const int h = (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T));
+        head = h < n ? h : n;
+        nvec = (n - head) / N;
+        tail = n - head - nvec * N;
     }
-    const T *x = row_at(logits, a, r);
-    float m = NEG_INF_F;
-    for (int i = tid; i < a.V; i += 256) m = fmaxf(m, (float)x[i]);
-    m = wave_max(m);
-    if (lane == 0) s_f[wave] = m;
+    // the scalar of thread `tid` (one at most), or -1
+    __device__ __forceinline__ int edge(int tid) const {
+        if (tid < head) return tid;
+        if (tid < head + tail) return head + nvec * VocabElem<T>::N + (tid - head);
+        return -1;
+    }
+};
+
+constexpr int MAX_KEYS = 1024;  // candidates that a workgroup sorts
+
+template <int NT>
+struct Shared {
+    static constexpr int NW = NT / 64;
+    float max[NW], tau[NW], z[NW], s[NW];
+    int count[NW];
+    int n;
+    unsigned long long key[MAX_KEYS];
+};
+
+template <int NT>
+__device__ __forceinline__ int block_count(int v, Shared<NT> &sh, int tid) {
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     __syncthreads();
-    m = fmaxf(fmaxf(s_f[0], s_f[1]), fmaxf(s_f[2], s_f[3]));
-    const bool empty = m == NEG_INF_F;
-    if (empty) m = 0.f;
+    if ((tid & 63) == 0) sh.count[tid >> 6] = v;
+    __syncthreads();
+    int t = 0;
+    for (int w = 0; w < Shared<NT>::NW; w++) t += sh.count[w];
+    return t;
+}
+
+// Calls f(value, index) for the elements of a span, reading them from memory.
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void for_each(const T *x, const Span<T> &sp, int tid, F f) {
+    constexpr int N = VocabElem<T>::N;
+    const int e = sp.edge(tid);
+    if (e >= 0) f((float)x[e], e);
+    const vec16 *xv = reinterpret_cast<const vec16 *>(x + sp.head);
+    for (int c = tid; c < sp.nvec; c += NT) {
+        float o[N];
+        VocabElem<T>::unpack(xv[c], o);
+        for (int i = 0; i < N; i++) f(o[i], sp.head + c * N + i);
+    }
+}
+
+// The `want` largest of a span whatever it holds (NaN, a constant, a mask that leaves fewer than `want`): the threshold t,
+// the want-th largest in the order of `order_of`, bit by bit - `guess` first, which is it where most of the span is one
+// value -, then everything above t (fewer than `want`), then the lowest indexes of those equal to t.  Reads the span again
+// for each step; rows of ordinary logits never come here.  Leaves `want` keys in sh.key.
+template <typename T, int NT>
+__device__ __forceinline__ void select_any(const T *x, const Span<T> &sp, int base, int want, unsigned guess, Shared<NT> &sh, int tid) {
+    constexpr int N = VocabElem<T>::N;
+    const auto count_from = [&](unsigned t) {
+        int k = 0;
+        for_each<T, NT>(x, sp, tid, [&](float v, int) { k += order_of(v) >= t ? 1 : 0; });
+        return block_count<NT>(k, sh, tid);
+    };
+    unsigned t = 0;
+    if (count_from(guess) >= want && (guess == 0xFFFFFFFFu || count_from(guess + 1) < want)) {
+        t = guess;
+    } else {
+        for (unsigned bit = 0x80000000u; bit != 0; bit >>= 1)
+            if (count_from(t | bit) >= want) t |= bit;
+    }
+    __syncthreads();
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    for_each<T, NT>(x, sp, tid, [&](float v, int i) {
+        if (order_of(v) > t) sh.key[atomicAdd(&sh.n, 1)] = key_of(v, base + i);
+    });
+    __syncthreads();
+    int n = sh.n;
+    // ties in ascending index: the head, rounds of one chunk a thread, the tail
+    const vec16 *xv = reinterpret_cast<const vec16 *>(x + sp.head);
+    const int rounds = (sp.nvec + NT - 1) / NT;
+    for (int round = -1; round <= rounds && n < want; round++) {
+        float o[N];
+        int first = 0, have = 0;
+        if (round == -1 || round == rounds) {
+            first = round == -1 ? tid : sp.head + sp.nvec * N + tid;
+            have = tid < (round == -1 ? sp.head : sp.tail) ? 1 : 0;
+            if (have) o[0] = (float)x[first];
+        } else if (tid + round * NT < sp.nvec) {
+            first = sp.head + (tid + round * NT) * N;
+            have = N;
+            VocabElem<T>::unpack(xv[tid + round * NT], o);
+        }
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) mine += i < have && order_of(o[i]) == t ? 1 : 0;
+        int upto = mine;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int w = __shfl_up(upto, d);
+            if ((tid & 63) >= d) upto += w;
+        }
+        __syncthreads();
+        if ((tid & 63) == 63) sh.count[tid >> 6] = upto;
+        __syncthreads();
+        int before = upto - mine, all = 0;
+        for (int w = 0; w < Shared<NT>::NW; w++) {
+            if (w < (tid >> 6)) before += sh.count[w];
+            all += sh.count[w];
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i < have && order_of(o[i]) == t) {
+                if (n + before < want) sh.key[n + before] = key_of(o[i], base + first + i);
+                before++;
+            }
+        n += all;
+        __syncthreads();
+    }
+}
+
+// What one workgroup finds in its part of a row.
+struct Part {
+    float m, z, s;  // maximum, sum of exp(x - m), sum of exp(x - m) (x - m); m = -inf, z = 0 where there is nothing
+};
+
+// One workgroup of NT threads over n elements at x, with up to MAXC chunks of 16 bytes a thread in registers: memory is
+// read once, all loads on their way together.
+//
+// The candidates for the alternatives come with the maximum: of every wave the q-th largest of its lanes' maxima
+// (q = top / waves, rounded up), the lowest of them over the waves: at least `top` elements lie at or above it, and of
+// ordinary logits hardly more (some 30 for 20 of 40000), which are collected beside the sums and put in order by
+// counting.  What overflows the list (a constant, a mask) or holds a NaN goes to select_any.
+// Leaves in sh.key[0..min(top, n)) the keys of the largest, unordered beyond that, their number in `kept`.
+template <typename T, int NT, int MAXC>
+__device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, bool keep, Shared<NT> &sh, int tid, int &kept) {
+    constexpr int N = VocabElem<T>::N;
+    constexpr int NW = NT / 64;
+    constexpr float LOG2E = 1.4426950408889634f;
+    const Span<T> sp(x, n);
+    const int wave = tid >> 6, lane = tid & 63;
+    const vec16 *xv = reinterpret_cast<const vec16 *>(x + sp.head);
+    vec16 buf[MAXC];
+    if (keep) {  // the backward reads the row again: leave it in the memory-side cache
+#pragma unroll
+        for (int i = 0; i < MAXC; i++) {
+            buf[i] = minus_infinities<T>();
+            if (tid + i * NT < sp.nvec) buf[i] = xv[tid + i * NT];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < MAXC; i++) {
+            buf[i] = minus_infinities<T>();
+            if (tid + i * NT < sp.nvec) buf[i] = __builtin_nontemporal_load(xv + tid + i * NT);
+        }
+    }
+    const int ei = sp.edge(tid);
+    const float edge = ei >= 0 ? (float)x[ei] : NEG_INF_F;
+    if (tid == 0) sh.n = 0;
+
+    typename VocabElem<T>::Max mx;
+#pragma unroll
+    for (int i = 0; i < MAXC; i++)
+        if (i * NT < sp.nvec) mx.take(buf[i]);
+    const float mine = fmaxf(mx.value(), edge);
+    float m = wave_max(mine), tau = m;
+    if (top > 0) {
+        float rest = mine;
+        for (int q = (top + NW - 1) / NW; q > 1; q--) {
+            rest = rest == tau ? NEG_INF_F : rest;
+            tau = wave_max(rest);
+        }
+    }
+    if (lane == 0) {
+        sh.max[wave] = m;
+        sh.tau[wave] = tau;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        m = fmaxf(m, sh.max[w]);
+        tau = fminf(tau, sh.tau[w]);
+    }
+    const float mm = m == NEG_INF_F ? 0.f : m;
+
+    const auto candidate = [&](float v, int i) {
+        if (v >= tau) {
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < MAX_KEYS) sh.key[at] = key_of(v, base + i);
+        }
+    };
     float z = 0.f, s = 0.f;
-    for (int i = tid; i < a.V; i += 256) {
-        const float d = (float)x[i] - m, e = __expf(d);
-        z += e;
-        s += e * fmaxf(d, -1e30f);
+    if (ei >= 0) {
+        const float d = edge - mm, e = __builtin_amdgcn_exp2f(d * LOG2E);
+        z = e;
+        s = e * fmaxf(d, -1e30f);
+        if (top > 0) candidate(edge, ei);
+    }
+#pragma unroll
+    for (int i = 0; i < MAXC; i++) {
+        if (i * NT < sp.nvec) {
+            float o[N];
+            opaque(buf[i]);
+            VocabElem<T>::unpack(buf[i], o);
+            float big = o[0];
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const float d = o[k] - mm, e = __builtin_amdgcn_exp2f(d * LOG2E);
+                z += e;
+                s = __builtin_fmaf(e, fmaxf(d, -1e30f), s);
+                big = fmaxf(big, o[k]);
+            }
+            if (top > 0 && big >= tau && tid + i * NT < sp.nvec) {
+#pragma unroll
+                for (int k = 0; k < N; k++) candidate(o[k], sp.head + (tid + i * NT) * N + k);
+            }
+        }
     }
     z = wave_sum(z);
     s = wave_sum(s);
-    __syncthreads();
     if (lane == 0) {
-        s_f[wave] = z;
-        s_f[4 + wave] = s;
+        sh.z[wave] = z;
+        sh.s[wave] = s;
     }
     __syncthreads();
-    z = (s_f[0] + s_f[1]) + (s_f[2] + s_f[3]);
-    s = (s_f[4] + s_f[5]) + (s_f[6] + s_f[7]);
-    const bool none = z == 0.f;  // nothing but -inf (a NaN makes z NaN)
-    const float lz = logf(z), H = none ? 0.f : lz - s / z;
+    z = sh.z[0];
+    s = sh.s[0];
+#pragma unroll
+    for (int w = 1; w < NW; w++) {
+        z += sh.z[w];
+        s += sh.s[w];
+    }
+    if (top > 0) {
+        kept = sh.n;
+        if (kept > MAX_KEYS || z != z) {  // (the same for every thread)
+            kept = top < n ? top : n;
+            select_any<T, NT>(x, sp, base, kept, order_of(tau), sh, tid);
+        }
+    }
+    return Part{m, z, s};
+}
+
+// The results of a row but its alternatives, by one thread.
+__device__ __forceinline__ void write_row(const LogprobArgs &a, int64_t r, int64_t tok, float x_tok, float mm, float lz, float H, bool none) {
+    if (a.tokens) a.logprobs[r] = tok >= a.V ? __builtin_nanf("") : none ? NEG_INF_F : (x_tok - mm) - lz;
+    if (a.entropy) a.entropy[r] = H;
+    if (a.stats) {
+        a.stats[r] = mm;
+        a.stats[a.rows + r] = lz;
+        a.stats[2 * a.rows + r] = H;
+    }
+}
+__device__ __forceinline__ void write_left_out(const LogprobArgs &a, int64_t r, int tid) {
     if (tid == 0) {
-        if (a.tokens) a.logprobs[r] = tok >= a.V ? __builtin_nanf("") : none ? NEG_INF_F : ((float)x[tok] - m) - lz;
-        if (a.entropy) a.entropy[r] = H;
-        if (a.stats) {
-            a.stats[r] = m;
-            a.stats[a.rows + r] = lz;
-            a.stats[2 * a.rows + r] = H;
+        a.logprobs[r] = 0.f;
+        if (a.entropy) a.entropy[r] = 0.f;
+    }
+    for (int k = tid; k < a.top; k += 64) {
+        a.top_logprobs[r * a.top + k] = NEG_INF_F;
+        a.top_tokens[r * a.top + k] = -1;
+    }
+}
+// The place of a key among n: how many are larger.
+__device__ __forceinline__ int rank_of(unsigned long long key, const unsigned long long *keys, int n) {
+    int rank = 0;
+    for (int j = 0; j < n; j++) rank += keys[j] > key ? 1 : 0;
+    return rank;
+}
+
+// A workgroup per row.
+template <typename T, int NT, int MAXC>
+__global__ __launch_bounds__(NT) void logprobs_kernel(const T *__restrict__ logits, LogprobArgs a) {
+    __shared__ Shared<NT> sh;
+    const unsigned r = blockIdx.x;
+    const int tid = threadIdx.x;
+    const int64_t tok = a.tokens ? a.tokens[r] : 0;
+    if (tok < 0) {
+        if (tid < 64) write_left_out(a, r, tid);
+        return;
+    }
+    const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows);
+    const float x_tok = tok < a.V ? (float)x[tok] : 0.f;
+    int kept = 0;
+    const Part p = scan_part<T, NT, MAXC>(x, a.V, 0, a.top, a.stats != nullptr, sh, tid, kept);
+    const bool none = p.z == 0.f;  // nothing but -inf (a NaN makes z NaN)
+    const float mm = none ? 0.f : p.m, lz = logf(p.z), H = none ? 0.f : lz - p.s / p.z;
+    if (tid == 0) write_row(a, r, tok, x_tok, mm, lz, H, none);
+    for (int i = tid; i < kept; i += NT) {
+        const unsigned long long key = sh.key[i];
+        const int k = rank_of(key, sh.key, kept);
+        if (k < a.top) {
+            const int at = index_of(key);
+            a.top_tokens[(int64_t)r * a.top + k] = at;
+            a.top_logprobs[(int64_t)r * a.top + k] = none ? NEG_INF_F : (value_of(key) - mm) - lz;
         }
     }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < a.top; k++) {
-        unsigned long long best = 0;
-        for (int i = tid; i < a.V; i += 256) {
-            const unsigned long long key = key_of((float)x[i], i);
-            if (key < last && key > best) best = key;
-        }
-        best = wave_max_key(best);
-        __syncthreads();
-        if (lane == 0) s_k[wave] = best;
-        __syncthreads();
-        for (int w = 0; w < 4; w++) best = s_k[w] > best ? s_k[w] : best;
-        last = best;
-        if (tid == 0) {
-            const float v = (float)x[index_of(best)];
-            a.top_logprobs[r * a.top + k] = none ? NEG_INF_F : (v - m) - lz;
-            a.top_tokens[r * a.top + k] = index_of(best);
+}
+
+// A row in several parts (few rows, or more than the registers of a workgroup hold): a workgroup each leaves its maximum,
+// sums and largest keys, in order, in the workspace ...
+template <typename T, int NT, int MAXC>
+__global__ __launch_bounds__(NT) void logprobs_part_kernel(const T *__restrict__ logits, LogprobArgs a, int part_len,
+                                                           unsigned long long *__restrict__ work) {
+    __shared__ Shared<NT> sh;
+    const unsigned r = blockIdx.x;
+    const int part = blockIdx.y, parts = gridDim.y, tid = threadIdx.x;
+    if (a.tokens && a.tokens[r] < 0) return;
+    const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows);
+    const int base = part * part_len;
+    const int n = a.V - base < part_len ? a.V - base : part_len;
+    int kept = 0;
+    const Part p = scan_part<T, NT, MAXC>(x + base, n, base, a.top, a.stats != nullptr, sh, tid, kept);
+    unsigned long long *out = work + ((int64_t)r * parts + part) * (2 + a.top);
+    if (tid == 0) {
+        out[0] = ((unsigned long long)__float_as_uint(p.z) << 32) | __float_as_uint(p.m);
+        out[1] = __float_as_uint(p.s);
+    }
+    for (int i = tid; i < kept; i += NT) {
+        const unsigned long long key = sh.key[i];
+        const int k = rank_of(key, sh.key, kept);
+        if (k < a.top) out[2 + k] = key;
+    }
+    for (int k = kept + tid; k < a.top; k += NT) out[2 + k] = 0;
+}
+
+// ... and a workgroup per row joins them: the sums are rescaled to the row's maximum, and of the parts' keys those at or
+// above the largest of the parts' last keys are put in order.
+constexpr int JOIN_NT = 256;
+constexpr int MAX_PARTS = 64;
+template <typename T>
+__global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restrict__ logits, LogprobArgs a, int parts,
+                                                                const unsigned long long *__restrict__ work) {
+    __shared__ unsigned long long s_key[MAX_PARTS * MAX_TOP];
+    __shared__ unsigned long long s_floor;
+    __shared__ int s_n;
+    const unsigned r = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int64_t tok = a.tokens ? a.tokens[r] : 0;
+    if (tok < 0) {
+        if (tid < 64) write_left_out(a, r, tid);
+        return;
+    }
+    const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows);
+    const float x_tok = tok < a.V ? (float)x[tok] : 0.f;
+    const int each = 2 + a.top;
+    const unsigned long long *in = work + (int64_t)r * parts * each;
+    // every wave forms the row's sums, lane by lane over the parts
+    float m_p = NEG_INF_F, z_p = 0.f, s_p = 0.f;
+    unsigned long long last = 0;
+    if (lane < parts) {
+        const unsigned long long zm = in[lane * each];
+        m_p = __uint_as_float((unsigned)zm);
+        z_p = __uint_as_float((unsigned)(zm >> 32));
+        s_p = __uint_as_float((unsigned)in[lane * each + 1]);
+        if (a.top > 0) last = in[lane * each + 1 + a.top];
+    }
+    const float m = wave_max(m_p), mm = m == NEG_INF_F ? 0.f : m;
+    float z = 0.f, s = 0.f;
+    if (z_p != 0.f) {  // (a part that holds a NaN makes z NaN)
+        const float d = fmaxf(m_p - mm, -1e30f), f = expf(d);
+        z = z_p * f;
+        s = f * (s_p + z_p * d);
+        if (m_p == __builtin_huge_valf()) z = __builtin_nanf("");
+    }
+    z = wave_sum(z);
+    s = wave_sum(s);
+    const bool none = z == 0.f;
+    const float lz = logf(z), H = none ? 0.f : lz - s / z;
+    if (tid == 0) write_row(a, r, tok, x_tok, mm, lz, H, none);
+    if (a.top == 0) return;
+    last = wave_max_key(last);
+    if (tid == 0) {
+        s_floor = last;
+        s_n = 0;
+    }
+    __syncthreads();
+    const unsigned long long floor = s_floor;
+    for (int i = tid; i < parts * a.top; i += JOIN_NT) {
+        const int p = i / a.top, k = i - p * a.top;
+        const unsigned long long key = in[p * each + 2 + k];
+        if (key != 0 && key >= floor) s_key[atomicAdd(&s_n, 1)] = key;
+    }
+    __syncthreads();
+    const int n = s_n;
+    for (int i = tid; i < n; i += JOIN_NT) {
+        const unsigned long long key = s_key[i];
+        const int k = rank_of(key, s_key, n);
+        if (k < a.top) {
+            a.top_tokens[(int64_t)r * a.top + k] = index_of(key);
+            a.top_logprobs[(int64_t)r * a.top + k] = none ? NEG_INF_F : (value_of(key) - mm) - lz;
         }
     }
+}
+
+// How a call is cut: parts of a row, and the registers of a workgroup.
+struct Cut {
+    int parts, len;
+};
+constexpr int BLOCKS_WANTED = 512;  // two workgroups for every CU
+constexpr int MIN_PART_BYTES = 8192;
+inline Cut cut_of(int es, int64_t rows, int64_t V) {
+    const int64_t chunk = 16 / es, most = (int64_t)512 * 10 * chunk;  // what a workgroup of 512 threads holds
+    int64_t parts = (V + most - 1) / most;
+    if (rows * parts < BLOCKS_WANTED && V * es > 2 * MIN_PART_BYTES) {
+        int64_t more = (BLOCKS_WANTED + rows - 1) / rows, fit = V * es / MIN_PART_BYTES;
+        if (fit < more) more = fit;
+        if (more > MAX_PARTS) more = MAX_PARTS;
+        if (more > parts) parts = more;
+    }
+    int64_t len = ((V + parts - 1) / parts + chunk - 1) / chunk * chunk;
+    parts = (V + len - 1) / len;
+    return Cut{(int)parts, (int)len};
+}
+
+template <typename T, int NT, int MAXC>
+void launch_rows(const T *x, const LogprobArgs &a, const Cut &c, unsigned long long *work, hipStream_t s) {
+    if (c.parts == 1) hipLaunchKernelGGL((logprobs_kernel<T, NT, MAXC>), dim3((unsigned)a.rows), dim3(NT), 0, s, x, a);
+    else
+        hipLaunchKernelGGL((logprobs_part_kernel<T, NT, MAXC>), dim3((unsigned)a.rows, (unsigned)c.parts), dim3(NT), 0, s, x, a, c.len, work);
+}
+template <typename T>
+int launch_forward(const void *logits, const LogprobArgs &a, void *work, hipStream_t s) {
+    const T *x = (const T *)logits;
+    const Cut c = cut_of((int)sizeof(T), a.rows, a.V);
+    const int chunks = (c.len + VocabElem<T>::N - 1) / VocabElem<T>::N;
+    unsigned long long *w = (unsigned long long *)work;
+    if (chunks <= 64 * 2) launch_rows<T, 64, 2>(x, a, c, w, s);
+    else if (chunks <= 256 * 4) launch_rows<T, 256, 4>(x, a, c, w, s);
+    else launch_rows<T, 512, 10>(x, a, c, w, s);
+    PCFGNAT_HIP_CHECK(hipGetLastError());
+    if (c.parts > 1) {
+        hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3((unsigned)a.rows), dim3(JOIN_NT), 0, s, x, a, c.parts, w);
+        PCFGNAT_HIP_CHECK(hipGetLastError());
+    }
+    return PCFGNAT_OK;
 }
 
 struct LogprobGradArgs {
@@ -180,7 +552,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(const T *__restrict_
 
 int check_sizes(const char *who, int dtype, int64_t outer, int64_t inner, int64_t so, int64_t si, int64_t V, int top) {
     PCFGNAT_REQUIRE(vocab_dtype_ok(dtype), "%s: logits must be float16, bfloat16 or float32", who);
-    PCFGNAT_REQUIRE(outer >= 0 && inner >= 0 && (outer == 0 || inner <= 2147483647 / outer) && V >= 1 && V <= (1 << 30) && so >= 0 && si >= 0,
+    PCFGNAT_REQUIRE(outer >= 0 && inner >= 0 && (outer == 0 || inner <= 2147483647 / outer) && V >= 1 && V <= MAX_LOGPROB_VOCAB && so >= 0 && si >= 0,
                     "%s: bad dimensions", who);
     PCFGNAT_REQUIRE(top >= 0 && top <= MAX_TOP && top <= V, "%s: between 0 and %d alternatives, at most the vocabulary (got %d of %lld)", who,
                     MAX_TOP, top, (long long)V);
@@ -193,11 +565,9 @@ int check_sizes(const char *who, int dtype, int64_t outer, int64_t inner, int64_
 using namespace pcfgnat;
 
 extern "C" size_t pcfgnat_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t V, int top) {
-    (void)dtype;
-    (void)rows;
-    (void)V;
-    (void)top;
-    return 0;
+    if (!vocab_dtype_ok(dtype) || rows <= 0 || V < 1 || V > MAX_LOGPROB_VOCAB || top < 0) return 0;
+    const Cut c = cut_of(vocab_elem_bytes(dtype), rows, V);
+    return c.parts == 1 ? 0 : (size_t)rows * c.parts * (2 + top) * 8;
 }
 
 extern "C" int pcfgnat_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer,
@@ -211,12 +581,10 @@ extern "C" int pcfgnat_token_logprobs(const void *logits, int dtype, int64_t out
     const int64_t rows = outer * inner;
     const LogprobArgs a{tokens, logprobs, entropy, top_logprobs, top_tokens, stats, rows, inner, stride_outer, stride_inner, (int)V, top};
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)rows), block(256);
-    if (dtype == PCFGNAT_F16) hipLaunchKernelGGL(logprobs_kernel<f16>, grid, block, 0, s, (const f16 *)logits, a);
-    else if (dtype == PCFGNAT_BF16) hipLaunchKernelGGL(logprobs_kernel<bf16>, grid, block, 0, s, (const bf16 *)logits, a);
-    else hipLaunchKernelGGL(logprobs_kernel<float>, grid, block, 0, s, (const float *)logits, a);
-    PCFGNAT_HIP_CHECK(hipGetLastError());
-    return PCFGNAT_OK;
+    PCFGNAT_REQUIRE(workspace || pcfgnat_token_logprobs_workspace_bytes(dtype, rows, V, top) == 0, "token_logprobs: null workspace");
+    if (dtype == PCFGNAT_F16) return launch_forward<f16>(logits, a, workspace, s);
+    if (dtype == PCFGNAT_BF16) return launch_forward<bf16>(logits, a, workspace, s);
+    return launch_forward<float>(logits, a, workspace, s);
 }
 
 extern "C" int pcfgnat_token_logprobs_backward(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer,
