@@ -7,6 +7,7 @@
 namespace pcfgnat {
 
 typedef unsigned int vec16 __attribute__((ext_vector_type(4)));  // one 16-byte global access
+typedef vec16 vec16_any __attribute__((aligned(2)));               // the same at the address of any element
 
 typedef _Float16 f16;
 typedef __bf16 bf16;

@@ -508,46 +508,105 @@ struct LogprobGradArgs {
     int V, top;
 };
 
-template <typename T>
-__global__ __launch_bounds__(256) void logprobs_grad_kernel(const T *__restrict__ logits, T *__restrict__ grad, LogprobGradArgs a) {
+// The gradient of one part of a row by one workgroup: NT threads, MAXC chunks of 16 bytes each, read once, written once.  The
+// chunks follow the alignment of the gradient's row; the logits' row may lie otherwise and is read unaligned.  The entries
+// at which something arrives besides (the token, the alternatives) are flagged by chunk in LDS, so that an ordinary chunk
+// pays one byte of LDS for them, and are added before the one rounding, in the order of the list.
+template <typename T, int NT, int MAXC>
+__global__ __launch_bounds__(NT) void logprobs_grad_kernel(const T *__restrict__ logits, T *__restrict__ grad, LogprobGradArgs a) {
+    constexpr int N = VocabElem<T>::N;
+    constexpr float LOG2E = 1.4426950408889634f;
     __shared__ float s_g[MAX_TOP + 1];
-    __shared__ int64_t s_i[MAX_TOP + 1];
-    const int64_t r = blockIdx.x;
+    __shared__ int s_i[MAX_TOP + 1];
+    __shared__ unsigned s_hit[NT * MAXC / 4];  // a byte for each chunk
+    const unsigned r = blockIdx.x;
     const int tid = threadIdx.x;
-    T *dx = grad + r * a.V;
+    const int base = blockIdx.y * (NT * MAXC * N), n = a.V - base < NT * MAXC * N ? a.V - base : NT * MAXC * N;
+    T *dx = grad + (int64_t)r * a.V + base;
+    const Span<T> sp(dx, n);
+    vec16 *dv = reinterpret_cast<vec16 *>(dx + sp.head);
     const int64_t tok = a.tokens ? a.tokens[r] : 0;
     const float lz = tok < 0 ? NEG_INF_F : a.stats[a.rows + r];
-    if (lz == NEG_INF_F) {
-        for (int i = tid; i < a.V; i += 256) dx[i] = (T)0.f;
+    const int ei = sp.edge(tid);
+    if (lz == NEG_INF_F) {  // left out, or nothing but -inf
+        const vec16 zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int i = 0; i < MAXC; i++)
+            if (tid + i * NT < sp.nvec) __builtin_nontemporal_store(zero, dv + tid + i * NT);
+        if (ei >= 0) dx[ei] = (T)0.f;
         return;
     }
-    const int64_t b = r / a.inner;
-    const T *x = logits + b * a.so + (r - b * a.inner) * a.si;
+    const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows) + base;
+    const vec16_any *xv = reinterpret_cast<const vec16_any *>(x + sp.head);
+    vec16 buf[MAXC];
+#pragma unroll
+    for (int i = 0; i < MAXC; i++)
+        if (tid + i * NT < sp.nvec) buf[i] = __builtin_nontemporal_load(xv + tid + i * NT);
+    const float edge = ei >= 0 ? (float)x[ei] : 0.f;
     const float m = a.stats[r], H = a.stats[2 * a.rows + r];
     const float gh = a.g_entropy ? a.g_entropy[r] : 0.f;
-    if (tid <= a.top) {
+    for (int i = tid; i < NT * MAXC / 4; i += NT) s_hit[i] = 0;
+    for (int k = tid; k <= a.top; k += NT) {
         float g = 0.f;
-        int64_t id = -1;
-        if (tid == 0 && a.g_logprobs) {
-            id = tok;
-            g = tok >= a.V ? __builtin_nanf("") : a.g_logprobs[r];
-        } else if (tid > 0 && a.g_top) {
-            id = a.top_tokens[r * a.top + tid - 1];
-            g = a.g_top[r * a.top + tid - 1];
+        int id = -1;
+        if (k == 0 && a.g_logprobs) {
+            id = tok < a.V ? (int)tok : -1;
+            g = tok < a.V ? a.g_logprobs[r] : __builtin_nanf("");
+        } else if (k > 0 && a.g_top) {
+            id = (int)a.top_tokens[(int64_t)r * a.top + k - 1];
+            g = a.g_top[(int64_t)r * a.top + k - 1];
         }
-        s_g[tid] = g;
-        s_i[tid] = id;
+        s_g[k] = g;
+        s_i[k] = id < 0 ? -1 : id - base;  // (negative: before this part)
     }
     __syncthreads();
-    float G = 0.f;
-    for (int k = 0; k <= a.top; k++) G += s_g[k];
-    for (int i = tid; i < a.V; i += 256) {
-        const float lp = ((float)x[i] - m) - lz;
-        float v = -__expf(lp) * (G + gh * (fmaxf(lp, -1e30f) + H));
-        for (int k = 0; k <= a.top; k++)
-            if (s_i[k] == i) v += s_g[k];
-        dx[i] = (T)v;
+    for (int k = tid; k <= a.top; k += NT) {
+        const int at = s_i[k] - sp.head;
+        if (at >= 0 && at < sp.nvec * N) atomicOr(&s_hit[at / N / 4], 1u << (8 * (at / N % 4)));
     }
+    __syncthreads();
+    float K = 0.f;
+    for (int k = 0; k <= a.top; k++) K += s_g[k];
+    K = __builtin_fmaf(gh, H, K);
+    const auto of = [&](float v) {
+        const float lp = (v - m) - lz;
+        return -__builtin_amdgcn_exp2f(lp * LOG2E) * __builtin_fmaf(gh, fmaxf(lp, -1e30f), K);
+    };
+    const auto arrivals = [&](float g, int at) {
+        for (int k = 0; k <= a.top; k++)
+            if (s_i[k] == at) g += s_g[k];
+        return g;
+    };
+    if (ei >= 0) dx[ei] = (T)arrivals(of(edge), ei);
+    const unsigned char *hit = reinterpret_cast<const unsigned char *>(s_hit);
+#pragma unroll
+    for (int i = 0; i < MAXC; i++) {
+        const int c = tid + i * NT;
+        if (c < sp.nvec) {
+            float o[N];
+            VocabElem<T>::unpack(buf[i], o);
+#pragma unroll
+            for (int k = 0; k < N; k++) o[k] = of(o[k]);
+            if (hit[c]) {
+#pragma unroll
+                for (int k = 0; k < N; k++) o[k] = arrivals(o[k], sp.head + c * N + k);
+            }
+            __builtin_nontemporal_store(VocabElem<T>::pack(o), dv + c);
+        }
+    }
+}
+
+template <typename T, int NT, int MAXC>
+void launch_grad_parts(const T *x, T *dx, const LogprobGradArgs &a, hipStream_t s) {
+    const int part = NT * MAXC * VocabElem<T>::N;
+    hipLaunchKernelGGL((logprobs_grad_kernel<T, NT, MAXC>), dim3((unsigned)a.rows, (unsigned)((a.V + part - 1) / part)), dim3(NT), 0, s, x, dx, a);
+}
+template <typename T>
+int launch_backward(const void *logits, void *grad, const LogprobGradArgs &a, hipStream_t s) {
+    if (a.V <= 64 * 2 * VocabElem<T>::N) launch_grad_parts<T, 64, 2>((const T *)logits, (T *)grad, a, s);
+    else launch_grad_parts<T, 256, 4>((const T *)logits, (T *)grad, a, s);
+    PCFGNAT_HIP_CHECK(hipGetLastError());
+    return PCFGNAT_OK;
 }
 
 int check_sizes(const char *who, int dtype, int64_t outer, int64_t inner, int64_t so, int64_t si, int64_t V, int top) {
@@ -599,11 +658,7 @@ extern "C" int pcfgnat_token_logprobs_backward(const void *logits, int dtype, in
     const int64_t rows = outer * inner;
     const LogprobGradArgs a{tokens, top_tokens, stats, grad_logprobs, grad_entropy, grad_top, rows, inner, stride_outer, stride_inner, (int)V, top};
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)rows), block(256);
-    if (dtype == PCFGNAT_F16) hipLaunchKernelGGL(logprobs_grad_kernel<f16>, grid, block, 0, s, (const f16 *)logits, (f16 *)grad_logits, a);
-    else if (dtype == PCFGNAT_BF16)
-        hipLaunchKernelGGL(logprobs_grad_kernel<bf16>, grid, block, 0, s, (const bf16 *)logits, (bf16 *)grad_logits, a);
-    else hipLaunchKernelGGL(logprobs_grad_kernel<float>, grid, block, 0, s, (const float *)logits, (float *)grad_logits, a);
-    PCFGNAT_HIP_CHECK(hipGetLastError());
-    return PCFGNAT_OK;
+    if (dtype == PCFGNAT_F16) return launch_backward<f16>(logits, grad_logits, a, s);
+    if (dtype == PCFGNAT_BF16) return launch_backward<bf16>(logits, grad_logits, a, s);
+    return launch_backward<float>(logits, grad_logits, a, s);
 }
