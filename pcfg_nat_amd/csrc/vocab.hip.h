@@ -23,6 +23,7 @@ struct ChunkMax {
 #pragma unroll
         for (int i = 0; i < (int)(16 / sizeof(T)); i++) m = fmaxf(m, (float)t[i]);
     }
+    __device__ __forceinline__ void take(const ChunkMax &o) { m = fmaxf(m, o.m); }
     __device__ __forceinline__ float value() const { return m; }
 };
 template <>
@@ -36,6 +37,7 @@ struct ChunkMax<f16> {
             m = __builtin_elementwise_max(m, __builtin_bit_cast(f16x2, pair));
         }
     }
+    __device__ __forceinline__ void take(const ChunkMax &o) { m = __builtin_elementwise_max(m, o.m); }
     __device__ __forceinline__ float value() const { return fmaxf((float)m.x, (float)m.y); }
 };
 

@@ -85,8 +85,8 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T *__restrict_
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------
-// Three launches, no atomics on results: the tokens in the order (token, position), sums over pieces of that order, joins of
-// the sums of a token whose run was cut.  The order is a function of the tokens alone, so are the sums.
+// Three launches, no atomics on results: the positions in an order that groups them by token (ascending within it), sums over
+// pieces of that order, joins of the sums of a token whose run was cut.  The order is a function of the tokens alone, so are the sums.
 //
 // What bounds it: writing all of dW (41 MB at 40000 x 512 float16, 6 us at the rate of a fill) and reading g once.  A decoder
 // input of a glanced graph holds one token in most places, so runs are cut evenly by position, not by token.
@@ -98,52 +98,63 @@ struct Plan {
 inline Plan plan_of(int64_t N, int64_t D) {
     // enough waves for the chip while pieces stay long enough that the cut runs' sums are few
     const int64_t waves = N * ((D + 511) / 512) / 2048;
-    int piece = 8;
+    int piece = 16;
     while (piece < 64 && piece * 2 <= waves) piece *= 2;
     return Plan{N, piece, (N + piece - 1) / piece};
 }
-// workspace: number of positions in the order (16 bytes), positions [N], tokens [N] in the order, sums of cut runs
-// [pieces][2][D] float32
+// workspace: number of positions in the order (16 bytes), positions [N], tokens [N] in the order, occurrences and begin of
+// each token [V], [V], sums of cut runs [pieces][2][D] float32
 inline size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 inline size_t order_bytes(const Plan &p) { return align16((size_t)p.N * 4); }
 
 constexpr int SORT_NT = 1024, SORT_NW = SORT_NT / 64;
-constexpr int MAX_STRIP = 1024;
+constexpr int MAX_OWN = 1024;  // tokens of the vocabulary that one workgroup owns, at the most
 
-// Every workgroup owns a strip of the vocabulary and looks for its tokens among all of them, each wave in its sixteenth of
-// the positions: first how often each occurs (and how many tokens lie below the strip, which is where the strip's part of
-// the order begins: no workgroup waits for another), then each to its place, in ascending position.  Lanes with the same
-// token take their places together.  The rows of the strip that no token selects are zeroed here.
-template <typename T>
+// Workgroup b of 2^block_bits owns the tokens b, b + 2^block_bits, ... of the vocabulary - spread, because vocabularies are
+// sorted by frequency: in strips the first workgroup would place half of all tokens (32768 tokens of 64000: 37 us in
+// strips) - and looks for them among all positions, each wave in its sixteenth: first how often each occurs
+// (and how many belong to the workgroups before this one, which is where its part of the order begins: no workgroup waits
+// for another), then each to its place, in ascending position.  The lanes that hold the same token are found by one ballot
+// for each bit of the token; the last of them moves the token's cursor on for all.  64 positions cost the same whether
+// they hold one token or 64.
 __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t *__restrict__ tokens, int64_t padding_idx, int N, int64_t V,
-                                                                  int strip, int64_t D, T *__restrict__ dweight, int *__restrict__ count,
+                                                                  int block_bits, int own_bits, int *__restrict__ count,
+                                                                  int *__restrict__ counts, int *__restrict__ starts,
                                                                   int *__restrict__ order_pos, int *__restrict__ order_tok) {
-    __shared__ int s_at[SORT_NW][MAX_STRIP];
-    __shared__ int s_total[MAX_STRIP];
+    __shared__ int s_at[SORT_NW][MAX_OWN];
     __shared__ int s_below[SORT_NW], s_wave[SORT_NW];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int64_t lo = (int64_t)blockIdx.x * strip;
-    const int ids = V - lo < strip ? (int)(V - lo) : strip;
+    const int block = (int)blockIdx.x, block_mask = (1 << block_bits) - 1;
+    const int ids = (int)((V - block + block_mask) >> block_bits);
     for (int i = lane; i < ids; i += 64) s_at[wave][i] = 0;
     const int groups = (N + 63) / 64, each = (groups + SORT_NW - 1) / SORT_NW;
     const int from = wave * each, to = from + each < groups ? from + each : groups;
-    // the token of a lane relative to the strip, or -1; tokens below the strip are counted
-    const auto local = [&](int g, int *below) {
-        const int64_t t = g * 64 + lane < N ? tokens[(int64_t)g * 64 + lane] : -1;
+    const auto load = [&](int g) -> int64_t {
+        const int64_t at = (int64_t)g * 64 + lane;
+        return g < to && at < N ? tokens[at] : -1;
+    };
+    // the token of a lane among the workgroup's own; -1 where it belongs to one before, -2 where to neither
+    const auto local = [&](int64_t t) {
         const bool real = t >= 0 && t < V && t != padding_idx;
-        if (below) *below += __popcll(__ballot(real && t < lo));
-        return real && t >= lo && t < lo + ids ? (int)(t - lo) : -1;
+        const int owner = (int)t & block_mask;
+        return !real || owner > block ? -2 : owner < block ? -1 : (int)(t >> block_bits);
     };
     int below = 0;
-    for (int g = from; g < to; g++) {
-        const int t = local(g, &below);
-        unsigned long long left = __ballot(t >= 0);
-        while (left) {
-            const int leader = __builtin_ctzll(left), id = __builtin_amdgcn_readlane(t, leader);
-            const unsigned long long same = __ballot(t == id);
-            if (lane == leader) s_at[wave][id] += __popcll(same);
-            left &= ~same;
+    unsigned long long found = 0;  // rounds of the first 64 that hold a token of this workgroup
+    constexpr int U = 8;
+    for (int g = from, round = 0; g < to; g += U, round++) {
+        int64_t t[U];
+        bool any = false;
+#pragma unroll
+        for (int u = 0; u < U; u++) t[u] = load(g + u);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int id = local(t[u]);
+            below += __popcll(__ballot(id == -1));
+            if (id >= 0) atomicAdd(&s_at[wave][id], 1);
+            any |= id >= 0;
         }
+        if (round < 64 && __ballot(any)) found |= 1ull << round;
     }
     if (lane == 0) s_below[wave] = below;
     __syncthreads();
@@ -158,11 +169,13 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
     }
     if (lane == 63) s_wave[wave] = upto;
     __syncthreads();
-    int base = upto - mine;
+    int base = upto - mine, all_before = 0, all_own = 0;
     for (int w = 0; w < SORT_NW; w++) {
-        base += s_below[w];
+        all_before += s_below[w];
         if (w < wave) base += s_wave[w];
+        all_own += s_wave[w];
     }
+    base += all_before;
     if (tid < ids) {
         int at = base;
         for (int w = 0; w < SORT_NW; w++) {
@@ -170,47 +183,60 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
             s_at[w][tid] = at;
             at += c;
         }
-        s_total[tid] = mine;
-        if (lo + tid == V - 1) *count = at;
+        counts[((int64_t)tid << block_bits) + block] = mine;
+        starts[((int64_t)tid << block_bits) + block] = base;
     }
+    if (block == block_mask && tid == 0) *count = all_before + all_own;
     __syncthreads();
-    for (int g = from; g < to; g++) {
-        const int t = local(g, nullptr);
-        unsigned long long left = __ballot(t >= 0);
-        while (left) {
-            const int leader = __builtin_ctzll(left), id = __builtin_amdgcn_readlane(t, leader);
-            const unsigned long long same = __ballot(t == id);
-            int at = 0;
-            if (lane == leader) at = atomicAdd(&s_at[wave][id], __popcll(same));
-            at = __builtin_amdgcn_readlane(at, leader) + __popcll(same & ((1ull << lane) - 1));
-            if (t == id) {
-                order_pos[at] = g * 64 + lane;
-                order_tok[at] = (int)(lo + id);
+    for (int g = from, round = 0; g < to; g += U, round++) {
+        if (round < 64 && !((found >> round) & 1)) continue;
+        int64_t t[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) t[u] = load(g + u);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int id = local(t[u]);
+            unsigned long long same = __ballot(id >= 0);
+            if (same == 0) continue;
+            for (int bit = 0; bit < own_bits; bit++) {
+                const unsigned long long set = __ballot((id >> bit) & 1);
+                same &= (id >> bit) & 1 ? set : ~set;
             }
-            left &= ~same;
+            if (id >= 0) {
+                // (the cursor of this wave alone; read by all lanes of the token before the last of them writes it)
+                const int at = __hip_atomic_load(&s_at[wave][id], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                const int rank = __popcll(same & ((1ull << lane) - 1)), all = __popcll(same);
+                if (rank == all - 1) __hip_atomic_store(&s_at[wave][id], at + all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                order_pos[at + rank] = (g + u) * 64 + lane;
+                order_tok[at + rank] = (int)t[u];
+            }
+            __builtin_amdgcn_wave_barrier();
         }
     }
-    const vec16 zero = {0u, 0u, 0u, 0u};
-    for (int i = wave; i < ids; i += SORT_NW)
-        if (s_total[i] == 0) {
-            T *row = dweight + (lo + i) * D;
-            for (int64_t c = (int64_t)lane * VocabElem<T>::N; c < D; c += 64 * VocabElem<T>::N) store_columns(row, c, D, zero);
-        }
 }
 
 // A wave sums one piece of the order over a tile of 64 chunks of columns, 8 rows of g on their way at a time.  Runs that begin
 // and end inside the piece are finished; the sums of the first and the last, where they go on outside, are left for the join.
+// The waves behind the last piece zero the rows that no token selects, beside the others' reads.
 constexpr int SUM_U = 8;
+constexpr int ZERO_ROWS = 8;  // rows that one of them looks at
 template <typename T>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(const T *__restrict__ g, int64_t gstride, float scale, T *__restrict__ dweight,
-                                                            int64_t D, int tiles, int piece, int64_t pieces, const int *__restrict__ count,
-                                                            const int *__restrict__ order_pos, const int *__restrict__ order_tok,
-                                                            float *__restrict__ cut) {
+                                                            int64_t D, int tiles, int piece, int64_t pieces, int64_t V, const int *__restrict__ count,
+                                                            const int *__restrict__ counts, const int *__restrict__ order_pos,
+                                                            const int *__restrict__ order_tok, float *__restrict__ cut) {
     constexpr int E = VocabElem<T>::N;
     const int64_t task = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int64_t p = task / tiles;
-    if (p >= pieces) return;
+    if (p >= pieces) {
+        const vec16 zero = {0u, 0u, 0u, 0u};
+        const int64_t v0 = (task - pieces * tiles) * ZERO_ROWS;
+        for (int64_t v = v0; v < v0 + ZERO_ROWS && v < V; v++)
+            if (counts[v] == 0)
+                for (int64_t c = (int64_t)lane * E; c < D; c += 64 * E) store_columns(dweight + v * D, c, D, zero);
+        return;
+    }
     const int total = *count;
     const int64_t c = ((task - p * tiles) * 64 + lane) * E;
     const int64_t from = p * piece;
@@ -263,42 +289,42 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const T *__restrict_
 }
 
 // Joins the sums of a run that begins in piece p and goes on behind it, in the order of the pieces: each wave of the workgroup
-// takes a stretch of them, the stretches are added in order.
-constexpr int JOIN_NW = 8;
+// takes a stretch of them, the stretches are added in order.  A workgroup covers 256 columns.
+constexpr int JOIN_NW = 4;
+typedef float float4_any __attribute__((ext_vector_type(4), aligned(4)));
 template <typename T>
-__global__ __launch_bounds__(JOIN_NW * 64) void embedding_join_kernel(float scale, T *__restrict__ dweight, int64_t D, int piece, int64_t pieces,
-                                                                      const int *__restrict__ count, const int *__restrict__ order_tok,
+__global__ __launch_bounds__(JOIN_NW * 64) void embedding_join_kernel(float scale, T *__restrict__ dweight, int64_t D, int piece,
+                                                                      const int *__restrict__ count, const int *__restrict__ counts,
+                                                                      const int *__restrict__ starts, const int *__restrict__ order_tok,
                                                                       const float *__restrict__ cut) {
-    __shared__ float s_sum[JOIN_NW][64];
-    const int64_t p = blockIdx.x, from = p * piece, end = from + piece;
+    __shared__ float4_any s_sum[JOIN_NW][64];
+    const int64_t p = blockIdx.x, end = (p + 1) * piece;
     const int total = *count, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (end >= total) return;
-    const int tok = order_tok[end];
-    if (order_tok[end - 1] != tok) return;                                                    // nothing goes on
-    if (order_tok[from] == tok && from > 0 && order_tok[from - 1] == tok) return;             // it began before
-    // pieces behind p that the run reaches: those whose first position holds its token
-    int64_t reach = 0;
-    for (int64_t q = p + 1;; q += 64) {
-        const bool in = q + lane < pieces && (q + lane) * piece < total && order_tok[(q + lane) * piece] == tok;
-        const unsigned long long out = ~__ballot(in);
-        reach += out ? __builtin_ctzll(out) : 64;
-        if (out) break;
-    }
+    const int tok = order_tok[end], start = starts[tok], behind = start + counts[tok];
+    if (start >= end || start < p * piece) return;  // it begins with the next piece, or began before this one
+    const int64_t reach = (behind - 1) / piece - p;  // pieces behind p that hold a part of the run
     const int64_t each = (reach + JOIN_NW - 1) / JOIN_NW, a = p + 1 + wave * each, b = a + each < p + 1 + reach ? a + each : p + 1 + reach;
-    for (int64_t c0 = (int64_t)blockIdx.y * 64; c0 < D; c0 += (int64_t)gridDim.y * 64) {
-        const int64_t c = c0 + lane;
-        float acc = 0.f;
-        if (c < D) {
-            if (wave == 0) acc = cut[(p * 2 + 1) * D + c];
+    for (int64_t c0 = (int64_t)blockIdx.y * 256; c0 < D; c0 += (int64_t)gridDim.y * 256) {
+        const int64_t c = c0 + lane * 4;
+        float4_any acc = {0.f, 0.f, 0.f, 0.f};
+        const auto add = [&](const float *sum) {
+            if (c + 4 <= D) acc += *reinterpret_cast<const float4_any *>(sum + c);
+            else
+                for (int k = 0; k < 3; k++)
+                    if (c + k < D) acc[k] += sum[c + k];
+        };
+        if (wave == 0) add(cut + (p * 2 + 1) * D);
 #pragma unroll 8
-            for (int64_t q = a; q < b; q++) acc += cut[q * 2 * D + c];
-        }
+        for (int64_t q = a; q < b; q++) add(cut + q * 2 * D);
         s_sum[wave][lane] = acc;
         __syncthreads();
-        if (wave == 0 && c < D) {
+        if (wave == 0) {
 #pragma unroll
             for (int w = 1; w < JOIN_NW; w++) acc += s_sum[w][lane];
-            dweight[(int64_t)tok * D + c] = (T)(acc * scale);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (c + k < D) dweight[(int64_t)tok * D + c + k] = (T)(acc[k] * scale);
         }
         __syncthreads();
     }
@@ -319,24 +345,27 @@ int backward(const void *g, int64_t gstride, const int64_t *tokens, float scale,
              int64_t N, int64_t V, int64_t D, hipStream_t s) {
     const Plan p = plan_of(N, D);
     const int tiles = (int)((D + 64 * VocabElem<T>::N - 1) / (64 * VocabElem<T>::N));
-    const int64_t sum_blocks = (p.pieces * tiles + 3) / 4;
+    const int64_t sum_blocks = (p.pieces * tiles + (V + ZERO_ROWS - 1) / ZERO_ROWS + 3) / 4;
     PCFGNAT_REQUIRE(sum_blocks <= 2147483647, "token_embedding_backward: the gradient is too large for one call");
     char *w = (char *)workspace;
     int *count = (int *)w, *order_pos = (int *)(w + 16), *order_tok = (int *)(w + 16 + order_bytes(p));
-    float *cut = (float *)(w + 16 + 2 * order_bytes(p));
-    int64_t strip = (V + 255) / 256;
-    strip = strip < 16 ? 16 : strip > MAX_STRIP ? MAX_STRIP : strip;
-    hipLaunchKernelGGL(embedding_order_kernel<T>, dim3((unsigned)((V + strip - 1) / strip)), dim3(SORT_NT), 0, s, tokens, padding_idx, (int)N, V,
-                       (int)strip, D, (T *)dweight, count, order_pos, order_tok);
+    int *counts = (int *)(w + 16 + 2 * order_bytes(p)), *starts = (int *)((char *)counts + align16((size_t)V * 4));
+    float *cut = (float *)((char *)starts + align16((size_t)V * 4));
+    // 256 workgroups, fewer for a small vocabulary (at least 16 tokens each), more for one beyond 256 * MAX_OWN
+    int block_bits = 0, own_bits = 0;
+    while (block_bits < 8 && (16 << (block_bits + 1)) <= V) block_bits++;
+    while (((V - 1) >> block_bits) + 1 > MAX_OWN) block_bits++;
+    while (((int64_t)1 << own_bits) < ((V - 1) >> block_bits) + 1) own_bits++;
+    hipLaunchKernelGGL(embedding_order_kernel, dim3(1u << block_bits), dim3(SORT_NT), 0, s, tokens, padding_idx, (int)N, V, block_bits, own_bits,
+                       count, counts, starts, order_pos, order_tok);
     PCFGNAT_HIP_CHECK(hipGetLastError());
-    if (N == 0) return PCFGNAT_OK;
     hipLaunchKernelGGL(embedding_sum_kernel<T>, dim3((unsigned)sum_blocks), dim3(256), 0, s, (const T *)g, gstride, scale, (T *)dweight, D,
-                       tiles, p.piece, p.pieces, count, order_pos, order_tok, cut);
+                       tiles, p.piece, p.pieces, V, count, counts, order_pos, order_tok, cut);
     PCFGNAT_HIP_CHECK(hipGetLastError());
     if (p.pieces > 1) {
-        const unsigned split = (unsigned)((D + 63) / 64 < 64 ? (D + 63) / 64 : 64);
+        const unsigned split = (unsigned)((D + 255) / 256 < 64 ? (D + 255) / 256 : 64);
         hipLaunchKernelGGL(embedding_join_kernel<T>, dim3((unsigned)p.pieces, split), dim3(JOIN_NW * 64), 0, s, scale, (T *)dweight, D, p.piece,
-                           p.pieces, count, order_tok, cut);
+                           count, counts, starts, order_tok, cut);
         PCFGNAT_HIP_CHECK(hipGetLastError());
     }
     return PCFGNAT_OK;
@@ -365,9 +394,9 @@ extern "C" int pcfgnat_token_embedding(const void *weight, int dtype, int64_t we
 }
 
 extern "C" size_t pcfgnat_token_embedding_backward_workspace_bytes(int64_t N, int64_t V, int64_t D) {
-    if (N < 0 || N > MAX_TOKENS || V < 1 || D < 1 || D > MAX_DIM) return 0;
+    if (N < 0 || N > MAX_TOKENS || V < 1 || V > MAX_VOCAB || D < 1 || D > MAX_DIM) return 0;
     const Plan p = plan_of(N, D);
-    return 16 + 2 * order_bytes(p) + align16((size_t)p.pieces * 2 * D * 4);
+    return 16 + 2 * order_bytes(p) + 2 * align16((size_t)V * 4) + align16((size_t)p.pieces * 2 * D * 4);
 }
 
 extern "C" int pcfgnat_token_embedding_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, float scale,

@@ -185,24 +185,29 @@ __device__ __forceinline__ void select_any(const T *x, const Span<T> &sp, int ba
     }
 }
 
-// What one workgroup finds in its part of a row.
+// What one workgroup finds in its part of a row, in base 2: z = sum of 2^t, s = sum of 2^t t, where t = (x - m) log2 e + shift.
+// (shift: the rounding of m log2 e, which the sums share and the results undo.)  m = -inf, z = 0 where there is nothing.
 struct Part {
-    float m, z, s;  // maximum, sum of exp(x - m), sum of exp(x - m) (x - m); m = -inf, z = 0 where there is nothing
+    float m, z, s, shift;
 };
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // One workgroup of NT threads over n elements at x, with up to MAXC chunks of 16 bytes a thread in registers: memory is
 // read once, all loads on their way together.
 //
-// The candidates for the alternatives come with the maximum: of every wave the q-th largest of its lanes' maxima
-// (q = top / waves, rounded up), the lowest of them over the waves: at least `top` elements lie at or above it, and of
-// ordinary logits hardly more (some 30 for 20 of 40000), which are collected beside the sums and put in order by
-// counting.  What overflows the list (a constant, a mask) or holds a NaN goes to select_any.
-// Leaves in sh.key[0..min(top, n)) the keys of the largest, unordered beyond that, their number in `kept`.
+// Sums: one fused multiply-add (which also widens a float16), one exponential, one addition and one multiply-add an
+// element.  Where an entry is -inf its t is too and s becomes NaN although z does not; such rows, and those whose maximum
+// is so large that m log2 e could leave float32, take the careful form, whose t is clamped.
+//
+// Alternatives: from every wave the q-th largest of its lanes' maxima (q = top / waves, rounded up), the lowest of them
+// over the waves: at least `top` elements lie at or above it, and of ordinary logits hardly more (some 30 for 20 of
+// 40000).  The chunks that hold one are known from the first pass's maxima; they alone are read again and their candidates
+// listed, to be put in order by counting.  What overflows the list (a constant, a mask) or holds a NaN goes to select_any.
+// Leaves in sh.key[0..kept) the keys of the candidates, all of the `top` largest among them.
 template <typename T, int NT, int MAXC>
 __device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, bool keep, Shared<NT> &sh, int tid, int &kept) {
     constexpr int N = VocabElem<T>::N;
     constexpr int NW = NT / 64;
-    constexpr float LOG2E = 1.4426950408889634f;
     const Span<T> sp(x, n);
     const int wave = tid >> 6, lane = tid & 63;
     const vec16 *xv = reinterpret_cast<const vec16 *>(x + sp.head);
@@ -224,10 +229,14 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, 
     const float edge = ei >= 0 ? (float)x[ei] : NEG_INF_F;
     if (tid == 0) sh.n = 0;
 
-    typename VocabElem<T>::Max mx;
+    typename VocabElem<T>::Max cm[MAXC], mx;
 #pragma unroll
-    for (int i = 0; i < MAXC; i++)
-        if (i * NT < sp.nvec) mx.take(buf[i]);
+    for (int i = 0; i < MAXC; i++) {
+        if (i * NT < sp.nvec) {
+            cm[i].take(buf[i]);
+            mx.take(cm[i]);
+        }
+    }
     const float mine = fmaxf(mx.value(), edge);
     float m = wave_max(mine), tau = m;
     if (top > 0) {
@@ -247,54 +256,79 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, 
         m = fmaxf(m, sh.max[w]);
         tau = fminf(tau, sh.tau[w]);
     }
+    if (top > 0) {
+        const auto candidate = [&](float v, int i) {
+            if (v >= tau) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < MAX_KEYS) sh.key[at] = key_of(v, base + i);
+            }
+        };
+        unsigned hold = 0;
+#pragma unroll
+        for (int i = 0; i < MAXC; i++)
+            if (i * NT < sp.nvec && cm[i].value() >= tau && tid + i * NT < sp.nvec) hold |= 1u << i;
+        if (ei >= 0) candidate(edge, ei);
+        while (hold) {
+            const int c = tid + __builtin_ctz(hold) * NT;
+            hold &= hold - 1;
+            const typename VocabElem<T>::vecT t = __builtin_bit_cast(typename VocabElem<T>::vecT, xv[c]);
+#pragma unroll
+            for (int k = 0; k < N; k++) candidate((float)t[k], sp.head + c * N + k);
+        }
+    }
     const float mm = m == NEG_INF_F ? 0.f : m;
-
-    const auto candidate = [&](float v, int i) {
-        if (v >= tau) {
-            const int at = atomicAdd(&sh.n, 1);
-            if (at < MAX_KEYS) sh.key[at] = key_of(v, base + i);
+    float z = 0.f, s = 0.f, shift = 0.f;
+    const auto sums = [&]() {  // over the workgroup
+        z = wave_sum(z);
+        s = wave_sum(s);
+        if (lane == 0) {
+            sh.z[wave] = z;
+            sh.s[wave] = s;
+        }
+        __syncthreads();
+        z = sh.z[0];
+        s = sh.s[0];
+#pragma unroll
+        for (int w = 1; w < NW; w++) {
+            z += sh.z[w];
+            s += sh.s[w];
         }
     };
-    float z = 0.f, s = 0.f;
-    if (ei >= 0) {
-        const float d = edge - mm, e = __builtin_amdgcn_exp2f(d * LOG2E);
-        z = e;
-        s = e * fmaxf(d, -1e30f);
-        if (top > 0) candidate(edge, ei);
-    }
+    bool careful = !(fabsf(mm) < 1e30f);
+    if (!careful) {
+        const float nb = -(mm * LOG2E);
+        shift = __builtin_fmaf(mm, LOG2E, nb);
+        if (ei >= 0) {
+            const float t = __builtin_fmaf(edge, LOG2E, nb);
+            z = __builtin_amdgcn_exp2f(t);
+            s = z * t;
+        }
 #pragma unroll
-    for (int i = 0; i < MAXC; i++) {
-        if (i * NT < sp.nvec) {
-            float o[N];
+        for (int i = 0; i < MAXC; i++) {
             opaque(buf[i]);
-            VocabElem<T>::unpack(buf[i], o);
-            float big = o[0];
+            if (tid + i * NT < sp.nvec) {
+                float o[N];
+                VocabElem<T>::unpack(buf[i], o);
 #pragma unroll
-            for (int k = 0; k < N; k++) {
-                const float d = o[k] - mm, e = __builtin_amdgcn_exp2f(d * LOG2E);
-                z += e;
-                s = __builtin_fmaf(e, fmaxf(d, -1e30f), s);
-                big = fmaxf(big, o[k]);
-            }
-            if (top > 0 && big >= tau && tid + i * NT < sp.nvec) {
-#pragma unroll
-                for (int k = 0; k < N; k++) candidate(o[k], sp.head + (tid + i * NT) * N + k);
+                for (int k = 0; k < N; k++) {
+                    const float t = __builtin_fmaf(o[k], LOG2E, nb), e = __builtin_amdgcn_exp2f(t);
+                    z += e;
+                    s = __builtin_fmaf(e, t, s);
+                }
             }
         }
+        sums();
+        careful = s != s && z == z;
+        if (careful) __syncthreads();
     }
-    z = wave_sum(z);
-    s = wave_sum(s);
-    if (lane == 0) {
-        sh.z[wave] = z;
-        sh.s[wave] = s;
-    }
-    __syncthreads();
-    z = sh.z[0];
-    s = sh.s[0];
-#pragma unroll
-    for (int w = 1; w < NW; w++) {
-        z += sh.z[w];
-        s += sh.s[w];
+    if (careful) {  // (the same for every thread)
+        z = s = shift = 0.f;
+        for_each<T, NT>(x, sp, tid, [&](float v, int) {
+            const float d = v - mm, e = __builtin_amdgcn_exp2f(d * LOG2E);
+            z += e;
+            s = __builtin_fmaf(e, fmaxf(d, -1e30f) * LOG2E, s);
+        });
+        sums();
     }
     if (top > 0) {
         kept = sh.n;
@@ -303,7 +337,7 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, 
             select_any<T, NT>(x, sp, base, kept, order_of(tau), sh, tid);
         }
     }
-    return Part{m, z, s};
+    return Part{m, z, s, shift};
 }
 
 // The results of a row but its alternatives, by one thread.
@@ -326,11 +360,20 @@ __device__ __forceinline__ void write_left_out(const LogprobArgs &a, int64_t r, 
         a.top_tokens[r * a.top + k] = -1;
     }
 }
-// The place of a key among n: how many are larger.
-__device__ __forceinline__ int rank_of(unsigned long long key, const unsigned long long *keys, int n) {
-    int rank = 0;
-    for (int j = 0; j < n; j++) rank += keys[j] > key ? 1 : 0;
-    return rank;
+// Calls f(key, place) for the keys whose place among the n in LDS - how many are larger - is below `top`; eight lanes count
+// for each key.
+template <int NT, typename F>
+__device__ __forceinline__ void in_order(const unsigned long long *keys, int n, int top, int tid, F f) {
+    for (int i0 = 0; i0 < n; i0 += NT / 8) {
+        const int i = i0 + (tid >> 3);
+        const unsigned long long key = i < n ? keys[i] : ~0ull;
+        int rank = 0;
+        for (int j = tid & 7; j < n; j += 8) rank += keys[j] > key ? 1 : 0;
+        rank += dpp_i<DPP_QUAD_XOR1>(rank);
+        rank += dpp_i<DPP_QUAD_XOR2>(rank);
+        rank += dpp_i<DPP_ROW_HALF_MIRROR>(rank);
+        if ((tid & 7) == 0 && i < n && rank < top) f(key, rank);
+    }
 }
 
 // A workgroup per row.
@@ -349,17 +392,12 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const T *__restrict__ logi
     int kept = 0;
     const Part p = scan_part<T, NT, MAXC>(x, a.V, 0, a.top, a.stats != nullptr, sh, tid, kept);
     const bool none = p.z == 0.f;  // nothing but -inf (a NaN makes z NaN)
-    const float mm = none ? 0.f : p.m, lz = logf(p.z), H = none ? 0.f : lz - p.s / p.z;
+    const float mm = none ? 0.f : p.m, l2 = log2f(p.z), lz = (l2 - p.shift) * LN2, H = none ? 0.f : (l2 - p.s / p.z) * LN2;
     if (tid == 0) write_row(a, r, tok, x_tok, mm, lz, H, none);
-    for (int i = tid; i < kept; i += NT) {
-        const unsigned long long key = sh.key[i];
-        const int k = rank_of(key, sh.key, kept);
-        if (k < a.top) {
-            const int at = index_of(key);
-            a.top_tokens[(int64_t)r * a.top + k] = at;
-            a.top_logprobs[(int64_t)r * a.top + k] = none ? NEG_INF_F : (value_of(key) - mm) - lz;
-        }
-    }
+    in_order<NT>(sh.key, kept, a.top, tid, [&](unsigned long long key, int k) {
+        a.top_tokens[(int64_t)r * a.top + k] = index_of(key);
+        a.top_logprobs[(int64_t)r * a.top + k] = none ? NEG_INF_F : (value_of(key) - mm) - lz;
+    });
 }
 
 // A row in several parts (few rows, or more than the registers of a workgroup hold): a workgroup each leaves its maximum,
@@ -379,18 +417,15 @@ __global__ __launch_bounds__(NT) void logprobs_part_kernel(const T *__restrict__
     unsigned long long *out = work + ((int64_t)r * parts + part) * (2 + a.top);
     if (tid == 0) {
         out[0] = ((unsigned long long)__float_as_uint(p.z) << 32) | __float_as_uint(p.m);
-        out[1] = __float_as_uint(p.s);
+        out[1] = ((unsigned long long)__float_as_uint(p.shift) << 32) | __float_as_uint(p.s);
     }
-    for (int i = tid; i < kept; i += NT) {
-        const unsigned long long key = sh.key[i];
-        const int k = rank_of(key, sh.key, kept);
-        if (k < a.top) out[2 + k] = key;
-    }
+    in_order<NT>(sh.key, kept, a.top, tid, [&](unsigned long long key, int k) { out[2 + k] = key; });
     for (int k = kept + tid; k < a.top; k += NT) out[2 + k] = 0;
 }
 
-// ... and a workgroup per row joins them: the sums are rescaled to the row's maximum, and of the parts' keys those at or
-// above the largest of the parts' last keys are put in order.
+// ... and a workgroup per row joins them: the sums are rescaled to the row's maximum, and the keys that can be among the
+// largest are put in order: those at or above every part's last key (its part alone has `top` of them) and at or above the
+// lowest of the parts' q-th keys (q = top / parts, rounded up: all parts together have).
 constexpr int JOIN_NT = 256;
 constexpr int MAX_PARTS = 64;
 template <typename T>
@@ -411,32 +446,38 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     const int each = 2 + a.top;
     const unsigned long long *in = work + (int64_t)r * parts * each;
     // every wave forms the row's sums, lane by lane over the parts
-    float m_p = NEG_INF_F, z_p = 0.f, s_p = 0.f;
-    unsigned long long last = 0;
+    float m_p = NEG_INF_F, z_p = 0.f, s_p = 0.f, shift_p = 0.f;
+    unsigned long long last = 0, below = 0;  // (below: all ones less the part's q-th key)
     if (lane < parts) {
         const unsigned long long zm = in[lane * each];
         m_p = __uint_as_float((unsigned)zm);
         z_p = __uint_as_float((unsigned)(zm >> 32));
-        s_p = __uint_as_float((unsigned)in[lane * each + 1]);
-        if (a.top > 0) last = in[lane * each + 1 + a.top];
+        const unsigned long long hs = in[lane * each + 1];
+        s_p = __uint_as_float((unsigned)hs);
+        shift_p = __uint_as_float((unsigned)(hs >> 32));
+        if (a.top > 0) {
+            last = in[lane * each + 1 + a.top];
+            below = ~in[lane * each + 1 + (a.top + parts - 1) / parts];
+        }
     }
     const float m = wave_max(m_p), mm = m == NEG_INF_F ? 0.f : m;
     float z = 0.f, s = 0.f;
     if (z_p != 0.f) {  // (a part that holds a NaN makes z NaN)
-        const float d = fmaxf(m_p - mm, -1e30f), f = expf(d);
+        // a part's t is larger than the row's by the rounding of its own maximum and by the distance of the two maxima
+        const float d = __builtin_fmaf(fmaxf(m_p - mm, -1e30f), LOG2E, -shift_p), f = exp2f(d);
         z = z_p * f;
         s = f * (s_p + z_p * d);
-        if (m_p == __builtin_huge_valf()) z = __builtin_nanf("");
     }
     z = wave_sum(z);
     s = wave_sum(s);
     const bool none = z == 0.f;
-    const float lz = logf(z), H = none ? 0.f : lz - s / z;
+    const float l2 = log2f(z), lz = l2 * LN2, H = none ? 0.f : (l2 - s / z) * LN2;
     if (tid == 0) write_row(a, r, tok, x_tok, mm, lz, H, none);
     if (a.top == 0) return;
     last = wave_max_key(last);
+    below = ~wave_max_key(below);
     if (tid == 0) {
-        s_floor = last;
+        s_floor = last > below ? last : below;
         s_n = 0;
     }
     __syncthreads();
@@ -448,14 +489,10 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     }
     __syncthreads();
     const int n = s_n;
-    for (int i = tid; i < n; i += JOIN_NT) {
-        const unsigned long long key = s_key[i];
-        const int k = rank_of(key, s_key, n);
-        if (k < a.top) {
-            a.top_tokens[(int64_t)r * a.top + k] = index_of(key);
-            a.top_logprobs[(int64_t)r * a.top + k] = none ? NEG_INF_F : (value_of(key) - mm) - lz;
-        }
-    }
+    in_order<JOIN_NT>(s_key, n, a.top, tid, [&](unsigned long long key, int k) {
+        a.top_tokens[(int64_t)r * a.top + k] = index_of(key);
+        a.top_logprobs[(int64_t)r * a.top + k] = none ? NEG_INF_F : (value_of(key) - mm) - lz;
+    });
 }
 
 // How a call is cut: parts of a row, and the registers of a workgroup.
@@ -515,7 +552,6 @@ struct LogprobGradArgs {
 template <typename T, int NT, int MAXC>
 __global__ __launch_bounds__(NT) void logprobs_grad_kernel(const T *__restrict__ logits, T *__restrict__ grad, LogprobGradArgs a) {
     constexpr int N = VocabElem<T>::N;
-    constexpr float LOG2E = 1.4426950408889634f;
     __shared__ float s_g[MAX_TOP + 1];
     __shared__ int s_i[MAX_TOP + 1];
     __shared__ unsigned s_hit[NT * MAXC / 4];  // a byte for each chunk
