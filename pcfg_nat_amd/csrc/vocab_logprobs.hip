@@ -14,7 +14,8 @@ namespace pcfgnat {
 namespace {
 
 constexpr int MAX_TOP = 64;
-constexpr int64_t MAX_LOGPROB_VOCAB = (int64_t)64 * 512 * 10 * 4;  // MAX_PARTS parts of what a workgroup holds, of float32
+constexpr int MAX_PARTS = 64;
+constexpr int64_t MAX_LOGPROB_VOCAB = (int64_t)MAX_PARTS * 512 * 20 * 4;  // of what a workgroup holds, of float32
 
 struct LogprobArgs {
     const int64_t *tokens;
@@ -39,10 +40,8 @@ __device__ __forceinline__ unsigned order_of(float x) {
 __device__ __forceinline__ unsigned long long key_of(float x, int i) {
     return ((unsigned long long)order_of(x) << 32) | (0xFFFFFFFEu - (unsigned)i);
 }
-__device__ __forceinline__ float value_of(unsigned long long key) {
-    const unsigned o = (unsigned)(key >> 32);
-    return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
-}
+__device__ __forceinline__ float value_of_order(unsigned o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o); }
+__device__ __forceinline__ float value_of(unsigned long long key) { return value_of_order((unsigned)(key >> 32)); }
 __device__ __forceinline__ int index_of(unsigned long long key) { return (int)(0xFFFFFFFEu - (unsigned)key); }
 
 __device__ __forceinline__ unsigned long long wave_max_key(unsigned long long v) {
@@ -80,11 +79,10 @@ struct Span {
     }
 };
 
-constexpr int MAX_KEYS = 1024;  // candidates that a workgroup sorts
-
 template <int NT>
 struct Shared {
     static constexpr int NW = NT / 64;
+    static constexpr int MAX_KEYS = NT == 64 ? 256 : 1024;  // candidates that the workgroup puts in order
     float max[NW], tau[NW], z[NW], s[NW];
     int count[NW];
     int n;
@@ -215,13 +213,11 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, 
     if (keep) {  // the backward reads the row again: leave it in the memory-side cache
 #pragma unroll
         for (int i = 0; i < MAXC; i++) {
-            buf[i] = minus_infinities<T>();
             if (tid + i * NT < sp.nvec) buf[i] = xv[tid + i * NT];
         }
     } else {
 #pragma unroll
         for (int i = 0; i < MAXC; i++) {
-            buf[i] = minus_infinities<T>();
             if (tid + i * NT < sp.nvec) buf[i] = __builtin_nontemporal_load(xv + tid + i * NT);
         }
     }
@@ -232,18 +228,34 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, 
     typename VocabElem<T>::Max cm[MAXC], mx;
 #pragma unroll
     for (int i = 0; i < MAXC; i++) {
-        if (i * NT < sp.nvec) {
-            cm[i].take(buf[i]);
-            mx.take(cm[i]);
-        }
+        if (tid + i * NT < sp.nvec) cm[i].take(buf[i]);
+        mx.take(cm[i]);
     }
-    const float mine = fmaxf(mx.value(), edge);
-    float m = wave_max(mine), tau = m;
-    if (top > 0) {
+    const float mine = max2_raw(mx.value(), edge);
+    float m = wave_max_raw(mine), tau = m;
+    if (NW == 1 && top > 12) {
+        // one wave and a long list: the top-th largest element itself, bit by bit over the registers (the lanes' maxima would
+        // take as many rounds as the list is long, and leave most of the row)
+        unsigned t = 0;
+        for (unsigned bit = 0x80000000u; bit != 0; bit >>= 1) {
+            const unsigned trial = t | bit;
+            int have = __popcll(__ballot(ei >= 0 && order_of(edge) >= trial));
+#pragma unroll
+            for (int i = 0; i < MAXC; i++) {
+                float o[N];
+                opaque(buf[i]);
+                VocabElem<T>::unpack(buf[i], o);
+#pragma unroll
+                for (int k = 0; k < N; k++) have += __popcll(__ballot(tid + i * NT < sp.nvec && order_of(o[k]) >= trial));
+            }
+            if (have >= top) t = trial;
+        }
+        tau = value_of_order(t);
+    } else if (top > 0) {
         float rest = mine;
         for (int q = (top + NW - 1) / NW; q > 1; q--) {
             rest = rest == tau ? NEG_INF_F : rest;
-            tau = wave_max(rest);
+            tau = wave_max_raw(rest);
         }
     }
     if (lane == 0) {
@@ -253,25 +265,33 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, 
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NW; w++) {
-        m = fmaxf(m, sh.max[w]);
-        tau = fminf(tau, sh.tau[w]);
+        m = max2_raw(m, sh.max[w]);
+        tau = sh.tau[w] < tau ? sh.tau[w] : tau;
     }
     if (top > 0) {
         const auto candidate = [&](float v, int i) {
             if (v >= tau) {
                 const int at = atomicAdd(&sh.n, 1);
-                if (at < MAX_KEYS) sh.key[at] = key_of(v, base + i);
+                if (at < Shared<NT>::MAX_KEYS) sh.key[at] = key_of(v, base + i);
             }
         };
+        if (ei >= 0) candidate(edge, ei);
         unsigned hold = 0;
 #pragma unroll
         for (int i = 0; i < MAXC; i++)
-            if (i * NT < sp.nvec && cm[i].value() >= tau && tid + i * NT < sp.nvec) hold |= 1u << i;
-        if (ei >= 0) candidate(edge, ei);
+            if (cm[i].value() >= tau && tid + i * NT < sp.nvec) hold |= 1u << i;
         while (hold) {
-            const int c = tid + __builtin_ctz(hold) * NT;
+            const int i = __builtin_ctz(hold), c = tid + i * NT;
             hold &= hold - 1;
-            const typename VocabElem<T>::vecT t = __builtin_bit_cast(typename VocabElem<T>::vecT, xv[c]);
+            typename VocabElem<T>::vecT t;
+            if (MAXC <= 4) {  // out of the registers (a choice among few); from memory, or its caches, where they are many
+                vec16 v = buf[0];
+#pragma unroll
+                for (int j = 1; j < MAXC; j++) v = i == j ? buf[j] : v;
+                t = __builtin_bit_cast(typename VocabElem<T>::vecT, v);
+            } else {
+                t = __builtin_bit_cast(typename VocabElem<T>::vecT, xv[c]);
+            }
 #pragma unroll
             for (int k = 0; k < N; k++) candidate((float)t[k], sp.head + c * N + k);
         }
@@ -332,7 +352,7 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, 
     }
     if (top > 0) {
         kept = sh.n;
-        if (kept > MAX_KEYS || z != z) {  // (the same for every thread)
+        if (kept > Shared<NT>::MAX_KEYS || z != z) {  // (the same for every thread)
             kept = top < n ? top : n;
             select_any<T, NT>(x, sp, base, kept, order_of(tau), sh, tid);
         }
@@ -427,7 +447,6 @@ __global__ __launch_bounds__(NT) void logprobs_part_kernel(const T *__restrict__
 // largest are put in order: those at or above every part's last key (its part alone has `top` of them) and at or above the
 // lowest of the parts' q-th keys (q = top / parts, rounded up: all parts together have).
 constexpr int JOIN_NT = 256;
-constexpr int MAX_PARTS = 64;
 template <typename T>
 __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restrict__ logits, LogprobArgs a, int parts,
                                                                 const unsigned long long *__restrict__ work) {
@@ -482,10 +501,13 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     }
     __syncthreads();
     const unsigned long long floor = s_floor;
-    for (int i = tid; i < parts * a.top; i += JOIN_NT) {
-        const int p = i / a.top, k = i - p * a.top;
-        const unsigned long long key = in[p * each + 2 + k];
-        if (key != 0 && key >= floor) s_key[atomicAdd(&s_n, 1)] = key;
+    for (int i0 = tid; i0 < parts * each; i0 += 8 * JOIN_NT) {  // (eight reads on their way; the parts' first two words are no keys)
+        unsigned long long key[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) key[u] = i0 + u * JOIN_NT < parts * each ? in[i0 + u * JOIN_NT] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+            if (key[u] != 0 && key[u] >= floor && (i0 + u * JOIN_NT) % each >= 2) s_key[atomicAdd(&s_n, 1)] = key[u];
     }
     __syncthreads();
     const int n = s_n;
@@ -495,24 +517,20 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     });
 }
 
-// How a call is cut: parts of a row, and the registers of a workgroup.
+// How a call is cut: parts of a row, each of at most MAX_CHUNKS chunks of 16 bytes.  A row that fits one workgroup's registers is
+// one part however few the rows are: a second launch for the join costs more than the larger workgroup (one row of 40000
+// float16: 6.4 us in one part, 8.6 us in nine; 100 rows: 7.8 and 11.2 us).
 struct Cut {
     int parts, len;
 };
-constexpr int BLOCKS_WANTED = 512;  // two workgroups for every CU
-constexpr int MIN_PART_BYTES = 8192;
-inline Cut cut_of(int es, int64_t rows, int64_t V) {
-    const int64_t chunk = 16 / es, most = (int64_t)512 * 10 * chunk;  // what a workgroup of 512 threads holds
-    int64_t parts = (V + most - 1) / most;
-    if (rows * parts < BLOCKS_WANTED && V * es > 2 * MIN_PART_BYTES) {
-        int64_t more = (BLOCKS_WANTED + rows - 1) / rows, fit = V * es / MIN_PART_BYTES;
-        if (fit < more) more = fit;
-        if (more > MAX_PARTS) more = MAX_PARTS;
-        if (more > parts) parts = more;
-    }
-    int64_t len = ((V + parts - 1) / parts + chunk - 1) / chunk * chunk;
-    parts = (V + len - 1) / len;
-    return Cut{(int)parts, (int)len};
+constexpr int MAX_CHUNKS = 512 * 20, PART_CHUNKS = 256 * 10;
+inline Cut cut_of(int es, int64_t V) {
+    const int64_t n = 16 / es, chunks = (V + n - 1) / n;
+    if (chunks <= MAX_CHUNKS) return Cut{1, (int)V};
+    int64_t parts = (chunks + PART_CHUNKS - 1) / PART_CHUNKS;
+    if (parts > MAX_PARTS) parts = MAX_PARTS;
+    const int64_t len = (chunks + parts - 1) / parts * n;
+    return Cut{(int)((V + len - 1) / len), (int)len};
 }
 
 template <typename T, int NT, int MAXC>
@@ -524,12 +542,17 @@ void launch_rows(const T *x, const LogprobArgs &a, const Cut &c, unsigned long l
 template <typename T>
 int launch_forward(const void *logits, const LogprobArgs &a, void *work, hipStream_t s) {
     const T *x = (const T *)logits;
-    const Cut c = cut_of((int)sizeof(T), a.rows, a.V);
+    const Cut c = cut_of((int)sizeof(T), a.V);
     const int chunks = (c.len + VocabElem<T>::N - 1) / VocabElem<T>::N;
     unsigned long long *w = (unsigned long long *)work;
+    // (every wave of a workgroup has to have elements: the alternatives' threshold is taken from all of them)
     if (chunks <= 64 * 2) launch_rows<T, 64, 2>(x, a, c, w, s);
+    else if (chunks <= 64 * 8) launch_rows<T, 64, 8>(x, a, c, w, s);
     else if (chunks <= 256 * 4) launch_rows<T, 256, 4>(x, a, c, w, s);
-    else launch_rows<T, 512, 10>(x, a, c, w, s);
+    else if (chunks <= 256 * 10) launch_rows<T, 256, 10>(x, a, c, w, s);
+    else if (chunks <= 512 * 10 && a.rows < 512) launch_rows<T, 512, 10>(x, a, c, w, s);
+    else if (chunks <= 256 * 20) launch_rows<T, 256, 20>(x, a, c, w, s);
+    else launch_rows<T, 512, 20>(x, a, c, w, s);
     PCFGNAT_HIP_CHECK(hipGetLastError());
     if (c.parts > 1) {
         hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3((unsigned)a.rows), dim3(JOIN_NT), 0, s, x, a, c.parts, w);
@@ -661,7 +684,7 @@ using namespace pcfgnat;
 
 extern "C" size_t pcfgnat_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t V, int top) {
     if (!vocab_dtype_ok(dtype) || rows <= 0 || V < 1 || V > MAX_LOGPROB_VOCAB || top < 0) return 0;
-    const Cut c = cut_of(vocab_elem_bytes(dtype), rows, V);
+    const Cut c = cut_of(vocab_elem_bytes(dtype), V);
     return c.parts == 1 ? 0 : (size_t)rows * c.parts * (2 + top) * 8;
 }
 
