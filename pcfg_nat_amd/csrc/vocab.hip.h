@@ -75,6 +75,7 @@ struct ChunkMax<f16> {
 template <typename T>
 struct VocabElem {
     static constexpr int N = 16 / (int)sizeof(T);
+    static constexpr unsigned LOWEST_BIT = sizeof(T) == 4 ? 1u : (float)(T)1.00390625f == 1.f ? 1u << 16 : 1u << 13;  // of the widened value
     typedef ChunkMax<T> Max;
     typedef T vecT __attribute__((ext_vector_type(N)));
     typedef float vecF __attribute__((ext_vector_type(N)));

@@ -33,8 +33,9 @@ __device__ __forceinline__ void store_columns(T *row, int64_t c, int64_t D, cons
 // The output is one run of N * D elements, written in aligned chunks of 16 bytes: a thread takes LOOKUP_U of them, finds the
 // row of each (one 64-bit division a workgroup, 32-bit ones from there), and has all its reads of the weight on their way
 // before the first store.  A chunk that lies across the end of a row (D no multiple of a chunk) goes element by element.
+// NARROW (here and below): rows shorter than a chunk.
 constexpr int LOOKUP_U = 4;
-template <typename T>
+template <typename T, bool NARROW>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T *__restrict__ weight, int64_t wstride, const int64_t *__restrict__ tokens,
                                                             float scale, T *__restrict__ out, int64_t N, int64_t V, unsigned D) {
     constexpr int E = VocabElem<T>::N;
@@ -43,22 +44,24 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T *__restrict_
     const unsigned col0 = (unsigned)(first - row0 * D);
     vec16 w[LOOKUP_U];
     int64_t tok[LOOKUP_U];
+    // (no branch around a load, whose result would be waited for at its end: what lies behind the output's end, across a row's
+    // end or outside the vocabulary reads some other place and is not used)
 #pragma unroll
     for (int u = 0; u < LOOKUP_U; u++) {
-        const unsigned at = (threadIdx.x + 256 * u) * E, in = col0 + at, row = in / D;
-        tok[u] = first + at < total ? tokens[row0 + row] : -1;
+        const unsigned at = (threadIdx.x + 256 * u) * E, row = (col0 + at) / D;
+        tok[u] = tokens[first + at < total ? row0 + row : N - 1];
     }
 #pragma unroll
     for (int u = 0; u < LOOKUP_U; u++) {
         const unsigned in = col0 + (threadIdx.x + 256 * u) * E, c = in - in / D * D;
-        if (tok[u] >= 0 && tok[u] < V && c + E <= D) w[u] = *reinterpret_cast<const vec16_any *>(weight + tok[u] * wstride + c);
+        if (!NARROW) w[u] = *reinterpret_cast<const vec16_any *>(weight + (tok[u] >= 0 && tok[u] < V ? tok[u] : 0) * wstride + (c + E <= D ? c : D - E));
     }
 #pragma unroll
     for (int u = 0; u < LOOKUP_U; u++) {
         const unsigned at = (threadIdx.x + 256 * u) * E, in = col0 + at, row = in / D, c = in - row * D;
         if (first + at >= total) continue;
         T *o = out + first + at;
-        if (c + E <= D) {
+        if (!NARROW && c + E <= D) {
             float f[E];
             if (tok[u] >= 0 && tok[u] < V) {
                 VocabElem<T>::unpack(w[u], f);
@@ -72,6 +75,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T *__restrict_
         } else {
             int64_t t = tok[u], r = row0 + row;
             unsigned cc = c;
+#pragma unroll 1
             for (int k = 0; k < E && first + at + k < total; k++) {
                 if (cc == D) {
                     cc = 0;
@@ -220,7 +224,7 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
 // The waves behind the last piece zero the rows that no token selects, beside the others' reads.
 constexpr int SUM_U = 8;
 constexpr int ZERO_ROWS = 8;  // rows that one of them looks at
-template <typename T>
+template <typename T, bool NARROW>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(const T *__restrict__ g, int64_t gstride, float scale, T *__restrict__ dweight,
                                                             int64_t D, int tiles, int piece, int64_t pieces, int64_t V, const int *__restrict__ count,
                                                             const int *__restrict__ counts, const int *__restrict__ order_pos,
@@ -238,21 +242,28 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const T *__restrict_
         return;
     }
     const int total = *count;
-    const int64_t c = ((task - p * tiles) * 64 + lane) * E;
     const int64_t from = p * piece;
     if (from >= total) return;
     const int n = total - from < piece ? (int)(total - from) : piece;
-    const int my_pos = lane < n ? order_pos[from + lane] : 0, my_tok = lane < n ? order_tok[from + lane] : -1;
-    const int before = from > 0 ? order_tok[from - 1] : -1, after = from + n < total ? order_tok[from + n] : -1;
+    const int my_pos = order_pos[from + (lane < n ? lane : 0)], my_tok = order_tok[from + (lane < n ? lane : 0)];
+    const int before = order_tok[from > 0 ? from - 1 : 0], after = order_tok[from + n < total ? from + n : from];
+    // Columns of a lane: the last ones of a row of D no multiple of a chunk are taken as the row's last whole chunk, whose first
+    // columns a neighbour sums and writes too, to the same values; narrower rows than a chunk go element by element.
+    const int64_t c0 = ((task - p * tiles) * 64 + lane) * E;
+    const bool live = c0 < D;
+    const int64_t c = NARROW ? 0 : c0 + E <= D ? c0 : D - E;
     float acc[E];
 #pragma unroll
     for (int k = 0; k < E; k++) acc[k] = 0.f;
-    bool opened_before = before == __builtin_amdgcn_readlane(my_tok, 0);
+    bool opened_before = from > 0 && before == __builtin_amdgcn_readlane(my_tok, 0);
     for (int j0 = 0; j0 < n; j0 += SUM_U) {
         vec16 buf[SUM_U];
 #pragma unroll
-        for (int u = 0; u < SUM_U; u++)
-            if (j0 + u < n && c < D) buf[u] = load_columns(g + (int64_t)__builtin_amdgcn_readlane(my_pos, j0 + u) * gstride, c, D);
+        for (int u = 0; u < SUM_U; u++) {  // (no branch around a load: the last row again behind the end)
+            const T *row = g + (int64_t)__builtin_amdgcn_readlane(my_pos, j0 + u < n ? j0 + u : n - 1) * gstride;
+            if (!NARROW) buf[u] = *reinterpret_cast<const vec16_any *>(row + c);
+            else buf[u] = load_columns(row, 0, D);
+        }
 #pragma unroll
         for (int u = 0; u < SUM_U; u++) {
             const int j = j0 + u;
@@ -262,21 +273,21 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const T *__restrict_
 #pragma unroll
                 for (int k = 0; k < E; k++) acc[k] += o[k];
                 const int tok = __builtin_amdgcn_readlane(my_tok, j);
-                const int next = j + 1 < n ? __builtin_amdgcn_readlane(my_tok, j + 1) : after;
                 const bool last = j + 1 == n;
-                if (next != tok || last) {
-                    const bool goes_on = last && next == tok;
-                    if (c < D) {
+                const bool goes_on = last ? from + n < total && after == tok : __builtin_amdgcn_readlane(my_tok, j + 1) == tok;
+                if (last || !goes_on) {
+                    if (live) {
                         if (opened_before || goes_on) {  // slot 0: a run from before (whether or not it ends here), slot 1: one that begins here
-                            float *to = cut + (p * 2 + (opened_before ? 0 : 1)) * D;
+                            float *to = cut + (p * 2 + (opened_before ? 0 : 1)) * D + c;
 #pragma unroll
                             for (int k = 0; k < E; k++)
-                                if (c + k < D) to[c + k] = acc[k];
+                                if (!NARROW || k < D) to[k] = acc[k];
                         } else {
                             float f[E];
 #pragma unroll
                             for (int k = 0; k < E; k++) f[k] = acc[k] * scale;
-                            store_columns(dweight + (int64_t)tok * D, c, D, VocabElem<T>::pack(f));
+                            if (NARROW) store_columns(dweight + (int64_t)tok * D, c, D, VocabElem<T>::pack(f));
+                            else *reinterpret_cast<vec16_any *>(dweight + (int64_t)tok * D + c) = VocabElem<T>::pack(f);
                         }
                     }
                     opened_before = false;
@@ -306,17 +317,20 @@ __global__ __launch_bounds__(JOIN_NW * 64) void embedding_join_kernel(float scal
     const int64_t reach = (behind - 1) / piece - p;  // pieces behind p that hold a part of the run
     const int64_t each = (reach + JOIN_NW - 1) / JOIN_NW, a = p + 1 + wave * each, b = a + each < p + 1 + reach ? a + each : p + 1 + reach;
     for (int64_t c0 = (int64_t)blockIdx.y * 256; c0 < D; c0 += (int64_t)gridDim.y * 256) {
-        const int64_t c = c0 + lane * 4;
+        // (the last columns of D no multiple of four: the row's last four, as in the sums)
+        const bool live = c0 + lane * 4 < D;
+        const int64_t c = D < 4 ? 0 : c0 + lane * 4 + 4 <= D ? c0 + lane * 4 : D - 4;
         float4_any acc = {0.f, 0.f, 0.f, 0.f};
-        const auto add = [&](const float *sum) {
-            if (c + 4 <= D) acc += *reinterpret_cast<const float4_any *>(sum + c);
-            else
-                for (int k = 0; k < 3; k++)
-                    if (c + k < D) acc[k] += sum[c + k];
-        };
-        if (wave == 0) add(cut + (p * 2 + 1) * D);
+        if (D >= 4) {
+            if (wave == 0) acc = *reinterpret_cast<const float4_any *>(cut + (p * 2 + 1) * D + c);
 #pragma unroll 8
-        for (int64_t q = a; q < b; q++) add(cut + q * 2 * D);
+            for (int64_t q = a; q < b; q++) acc += *reinterpret_cast<const float4_any *>(cut + q * 2 * D + c);
+        } else {
+            for (int k = 0; k < D; k++) {
+                if (wave == 0) acc[k] = cut[(p * 2 + 1) * D + k];
+                for (int64_t q = a; q < b; q++) acc[k] += cut[q * 2 * D + k];
+            }
+        }
         s_sum[wave][lane] = acc;
         __syncthreads();
         if (wave == 0) {
@@ -324,7 +338,7 @@ __global__ __launch_bounds__(JOIN_NW * 64) void embedding_join_kernel(float scal
             for (int w = 1; w < JOIN_NW; w++) acc += s_sum[w][lane];
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                if (c + k < D) dweight[(int64_t)tok * D + c + k] = (T)(acc[k] * scale);
+                if (live && c + k < D) dweight[(int64_t)tok * D + c + k] = (T)(acc[k] * scale);
         }
         __syncthreads();
     }
@@ -335,8 +349,12 @@ int forward(const void *weight, int64_t wstride, const int64_t *tokens, float sc
             hipStream_t s) {
     const int64_t each = 256 * LOOKUP_U * VocabElem<T>::N, blocks = (N * D + each - 1) / each;
     PCFGNAT_REQUIRE(blocks <= 2147483647, "token_embedding: the output is too large for one call");
-    hipLaunchKernelGGL(embedding_fwd_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, (const T *)weight, wstride, tokens, scale, (T *)out, N,
-                       V, (unsigned)D);
+    if (D < VocabElem<T>::N)
+        hipLaunchKernelGGL((embedding_fwd_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)weight, wstride, tokens, scale,
+                           (T *)out, N, V, (unsigned)D);
+    else
+        hipLaunchKernelGGL((embedding_fwd_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)weight, wstride, tokens, scale,
+                           (T *)out, N, V, (unsigned)D);
     PCFGNAT_HIP_CHECK(hipGetLastError());
     return PCFGNAT_OK;
 }
@@ -359,8 +377,12 @@ int backward(const void *g, int64_t gstride, const int64_t *tokens, float scale,
     hipLaunchKernelGGL(embedding_order_kernel, dim3(1u << block_bits), dim3(SORT_NT), 0, s, tokens, padding_idx, (int)N, V, block_bits, own_bits,
                        count, counts, starts, order_pos, order_tok);
     PCFGNAT_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL(embedding_sum_kernel<T>, dim3((unsigned)sum_blocks), dim3(256), 0, s, (const T *)g, gstride, scale, (T *)dweight, D,
-                       tiles, p.piece, p.pieces, V, count, counts, order_pos, order_tok, cut);
+    if (D < VocabElem<T>::N)
+        hipLaunchKernelGGL((embedding_sum_kernel<T, true>), dim3((unsigned)sum_blocks), dim3(256), 0, s, (const T *)g, gstride, scale,
+                           (T *)dweight, D, tiles, p.piece, p.pieces, V, count, counts, order_pos, order_tok, cut);
+    else
+        hipLaunchKernelGGL((embedding_sum_kernel<T, false>), dim3((unsigned)sum_blocks), dim3(256), 0, s, (const T *)g, gstride, scale,
+                           (T *)dweight, D, tiles, p.piece, p.pieces, V, count, counts, order_pos, order_tok, cut);
     PCFGNAT_HIP_CHECK(hipGetLastError());
     if (p.pieces > 1) {
         const unsigned split = (unsigned)((D + 255) / 256 < 64 ? (D + 255) / 256 : 64);

@@ -15,7 +15,7 @@ namespace {
 
 constexpr int MAX_TOP = 64;
 constexpr int MAX_PARTS = 64;
-constexpr int64_t MAX_LOGPROB_VOCAB = (int64_t)MAX_PARTS * 512 * 20 * 4;  // of what a workgroup holds, of float32
+constexpr int64_t MAX_LOGPROB_VOCAB = (int64_t)MAX_PARTS * 256 * 20 * 4;  // of what a part's workgroup holds, of float32
 
 struct LogprobArgs {
     const int64_t *tokens;
@@ -37,6 +37,7 @@ __device__ __forceinline__ unsigned order_of(float x) {
     const unsigned b = __float_as_uint(x + 0.f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+constexpr unsigned LOWEST_ORDER = 0x007FFFFFu;  // of -inf
 __device__ __forceinline__ unsigned long long key_of(float x, int i) {
     return ((unsigned long long)order_of(x) << 32) | (0xFFFFFFFEu - (unsigned)i);
 }
@@ -119,7 +120,7 @@ __device__ __forceinline__ void for_each(const T *x, const Span<T> &sp, int tid,
 // value -, then everything above t (fewer than `want`), then the lowest indexes of those equal to t.  Reads the span again
 // for each step; rows of ordinary logits never come here.  Leaves `want` keys in sh.key.
 template <typename T, int NT>
-__device__ __forceinline__ void select_any(const T *x, const Span<T> &sp, int base, int want, unsigned guess, Shared<NT> &sh, int tid) {
+__device__ __forceinline__ void select_any(const T *x, const Span<T> &sp, int want, unsigned guess, Shared<NT> &sh, int tid) {
     constexpr int N = VocabElem<T>::N;
     const auto count_from = [&](unsigned t) {
         int k = 0;
@@ -137,7 +138,7 @@ __device__ __forceinline__ void select_any(const T *x, const Span<T> &sp, int ba
     if (tid == 0) sh.n = 0;
     __syncthreads();
     for_each<T, NT>(x, sp, tid, [&](float v, int i) {
-        if (order_of(v) > t) sh.key[atomicAdd(&sh.n, 1)] = key_of(v, base + i);
+        if (order_of(v) > t) sh.key[atomicAdd(&sh.n, 1)] = key_of(v, i);
     });
     __syncthreads();
     int n = sh.n;
@@ -175,7 +176,7 @@ __device__ __forceinline__ void select_any(const T *x, const Span<T> &sp, int ba
 #pragma unroll
         for (int i = 0; i < N; i++)
             if (i < have && order_of(o[i]) == t) {
-                if (n + before < want) sh.key[n + before] = key_of(o[i], base + first + i);
+                if (n + before < want) sh.key[n + before] = key_of(o[i], first + i);
                 before++;
             }
         n += all;
@@ -202,55 +203,60 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // 40000).  The chunks that hold one are known from the first pass's maxima; they alone are read again and their candidates
 // listed, to be put in order by counting.  What overflows the list (a constant, a mask) or holds a NaN goes to select_any.
 // Leaves in sh.key[0..kept) the keys of the candidates, all of the `top` largest among them.
+// With `lanes` the alternatives are left to another launch: each lane leaves the maximum of its elements there.
 template <typename T, int NT, int MAXC>
-__device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, bool keep, Shared<NT> &sh, int tid, int &kept) {
+__device__ __forceinline__ Part scan_part(const T *x, int n, int top, bool keep, Shared<NT> &sh, int tid, int &kept, float *lanes) {
     constexpr int N = VocabElem<T>::N;
-    constexpr int NW = NT / 64;
+    constexpr int NW = NT / 64, FEW = 2;
     const Span<T> sp(x, n);
     const int wave = tid >> 6, lane = tid & 63;
     const vec16 *xv = reinterpret_cast<const vec16 *>(x + sp.head);
+    // (no branch around a load, whose result would be waited for at its end: threads behind the last chunk read that one again)
     vec16 buf[MAXC];
-    if (keep) {  // the backward reads the row again: leave it in the memory-side cache
+    const int ei = sp.edge(tid);
+    const T edge_raw = x[ei >= 0 ? ei : 0];
+    if (sp.nvec == 0) {
 #pragma unroll
-        for (int i = 0; i < MAXC; i++) {
-            if (tid + i * NT < sp.nvec) buf[i] = xv[tid + i * NT];
-        }
+        for (int i = 0; i < MAXC; i++) buf[i] = vec16{0u, 0u, 0u, 0u};
+    } else if (keep) {  // the backward reads the row again: leave it in the memory-side cache
+#pragma unroll
+        for (int i = 0; i < MAXC; i++) buf[i] = xv[tid + i * NT < sp.nvec ? tid + i * NT : sp.nvec - 1];
     } else {
 #pragma unroll
-        for (int i = 0; i < MAXC; i++) {
-            if (tid + i * NT < sp.nvec) buf[i] = __builtin_nontemporal_load(xv + tid + i * NT);
-        }
+        for (int i = 0; i < MAXC; i++) buf[i] = __builtin_nontemporal_load(xv + (tid + i * NT < sp.nvec ? tid + i * NT : sp.nvec - 1));
     }
-    const int ei = sp.edge(tid);
-    const float edge = ei >= 0 ? (float)x[ei] : NEG_INF_F;
     if (tid == 0) sh.n = 0;
 
     typename VocabElem<T>::Max cm[MAXC], mx;
 #pragma unroll
     for (int i = 0; i < MAXC; i++) {
-        if (tid + i * NT < sp.nvec) cm[i].take(buf[i]);
+        cm[i].take(buf[i]);
+        if (tid + i * NT >= sp.nvec) cm[i] = typename VocabElem<T>::Max();
         mx.take(cm[i]);
     }
+    const float edge = ei >= 0 ? (float)edge_raw : NEG_INF_F;
     const float mine = max2_raw(mx.value(), edge);
+    if (lanes != nullptr) lanes[tid] = mine;
     float m = wave_max_raw(mine), tau = m;
-    if (NW == 1 && top > 12) {
-        // one wave and a long list: the top-th largest element itself, bit by bit over the registers (the lanes' maxima would
-        // take as many rounds as the list is long, and leave most of the row)
+    if (NW == 1 && top > 24) {
+        // one wave and a long list: the top-th largest element itself, bit by bit over the registers, as far down as the type
+        // has bits (the lanes' maxima would leave a good part of the row)
         unsigned t = 0;
-        for (unsigned bit = 0x80000000u; bit != 0; bit >>= 1) {
-            const unsigned trial = t | bit;
-            int have = __popcll(__ballot(ei >= 0 && order_of(edge) >= trial));
+        for (unsigned bit = 0x80000000u; bit >= VocabElem<T>::LOWEST_BIT; bit >>= 1) {
+            const float trial = (t | bit) > LOWEST_ORDER ? value_of_order(t | bit) : NEG_INF_F;
+            int have = __popcll(__ballot(edge >= trial && ei >= 0));
 #pragma unroll
             for (int i = 0; i < MAXC; i++) {
                 float o[N];
                 opaque(buf[i]);
                 VocabElem<T>::unpack(buf[i], o);
+                const bool in = tid + i * NT < sp.nvec;
 #pragma unroll
-                for (int k = 0; k < N; k++) have += __popcll(__ballot(tid + i * NT < sp.nvec && order_of(o[k]) >= trial));
+                for (int k = 0; k < N; k++) have += __popcll(__ballot(o[k] >= trial && in));
             }
-            if (have >= top) t = trial;
+            if (have >= top) t |= bit;
         }
-        tau = value_of_order(t);
+        tau = t > LOWEST_ORDER ? value_of_order(t) : NEG_INF_F;
     } else if (top > 0) {
         float rest = mine;
         for (int q = (top + NW - 1) / NW; q > 1; q--) {
@@ -268,52 +274,18 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, 
         m = max2_raw(m, sh.max[w]);
         tau = sh.tau[w] < tau ? sh.tau[w] : tau;
     }
+    // chunks that hold a candidate: out of the registers where a thread has few, read again where it has many - the first
+    // one's read is on its way during the sums
+    unsigned hold = 0;
+    vec16 held = {0u, 0u, 0u, 0u};
     if (top > 0) {
-        const auto candidate = [&](float v, int i) {
-            if (v >= tau) {
-                const int at = atomicAdd(&sh.n, 1);
-                if (at < Shared<NT>::MAX_KEYS) sh.key[at] = key_of(v, base + i);
-            }
-        };
-        if (ei >= 0) candidate(edge, ei);
-        unsigned hold = 0;
 #pragma unroll
         for (int i = 0; i < MAXC; i++)
             if (cm[i].value() >= tau && tid + i * NT < sp.nvec) hold |= 1u << i;
-        while (hold) {
-            const int i = __builtin_ctz(hold), c = tid + i * NT;
-            hold &= hold - 1;
-            typename VocabElem<T>::vecT t;
-            if (MAXC <= 4) {  // out of the registers (a choice among few); from memory, or its caches, where they are many
-                vec16 v = buf[0];
-#pragma unroll
-                for (int j = 1; j < MAXC; j++) v = i == j ? buf[j] : v;
-                t = __builtin_bit_cast(typename VocabElem<T>::vecT, v);
-            } else {
-                t = __builtin_bit_cast(typename VocabElem<T>::vecT, xv[c]);
-            }
-#pragma unroll
-            for (int k = 0; k < N; k++) candidate((float)t[k], sp.head + c * N + k);
-        }
+        if (MAXC > FEW && hold) held = xv[tid + __builtin_ctz(hold) * NT];
     }
     const float mm = m == NEG_INF_F ? 0.f : m;
     float z = 0.f, s = 0.f, shift = 0.f;
-    const auto sums = [&]() {  // over the workgroup
-        z = wave_sum(z);
-        s = wave_sum(s);
-        if (lane == 0) {
-            sh.z[wave] = z;
-            sh.s[wave] = s;
-        }
-        __syncthreads();
-        z = sh.z[0];
-        s = sh.s[0];
-#pragma unroll
-        for (int w = 1; w < NW; w++) {
-            z += sh.z[w];
-            s += sh.s[w];
-        }
-    };
     bool careful = !(fabsf(mm) < 1e30f);
     if (!careful) {
         const float nb = -(mm * LOG2E);
@@ -337,24 +309,67 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int base, int top, 
                 }
             }
         }
-        sums();
-        careful = s != s && z == z;
-        if (careful) __syncthreads();
-    }
-    if (careful) {  // (the same for every thread)
-        z = s = shift = 0.f;
-        for_each<T, NT>(x, sp, tid, [&](float v, int) {
-            const float d = v - mm, e = __builtin_amdgcn_exp2f(d * LOG2E);
-            z += e;
-            s = __builtin_fmaf(e, fmaxf(d, -1e30f) * LOG2E, s);
-        });
-        sums();
     }
     if (top > 0) {
+        const auto take = [&](float v, int i) {
+            if (v >= tau) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < Shared<NT>::MAX_KEYS) sh.key[at] = key_of(v, i);
+            }
+        };
+        if (ei >= 0) take(edge, ei);
+        if (MAXC <= FEW) {
+#pragma unroll
+            for (int i = 0; i < MAXC; i++)
+                if (hold & (1u << i)) {
+                    const typename VocabElem<T>::vecT t = __builtin_bit_cast(typename VocabElem<T>::vecT, buf[i]);
+#pragma unroll
+                    for (int k = 0; k < N; k++) take((float)t[k], sp.head + (tid + i * NT) * N + k);
+                }
+        } else {
+            while (hold) {
+                const int c = tid + __builtin_ctz(hold) * NT;
+                const typename VocabElem<T>::vecT t = __builtin_bit_cast(typename VocabElem<T>::vecT, held);
+                hold &= hold - 1;
+                if (hold) held = xv[tid + __builtin_ctz(hold) * NT];
+#pragma unroll
+                for (int k = 0; k < N; k++) take((float)t[k], sp.head + c * N + k);
+            }
+        }
+    }
+    for (bool again = careful;;) {  // (everything here is the same for every thread)
+        if (again) {
+            z = s = shift = 0.f;
+            for_each<T, NT>(x, sp, tid, [&](float v, int) {
+                const float d = v - mm, e = __builtin_amdgcn_exp2f(d * LOG2E);
+                z += e;
+                s = __builtin_fmaf(e, fmaxf(d, -1e30f) * LOG2E, s);
+            });
+        }
+        z = wave_sum(z);
+        s = wave_sum(s);
+        if (lane == 0) {
+            sh.z[wave] = z;
+            sh.s[wave] = s;
+        }
+        __syncthreads();
+        z = sh.z[0];
+        s = sh.s[0];
+#pragma unroll
+        for (int w = 1; w < NW; w++) {
+            z += sh.z[w];
+            s += sh.s[w];
+        }
+        if (again || !(s != s && z == z)) break;
+        again = true;
+        __syncthreads();
+    }
+    if (top > 0) {
+        const int want = top < n ? top : n;
         kept = sh.n;
-        if (kept > Shared<NT>::MAX_KEYS || z != z) {  // (the same for every thread)
-            kept = top < n ? top : n;
-            select_any<T, NT>(x, sp, base, kept, order_of(tau), sh, tid);
+        if (kept > Shared<NT>::MAX_KEYS || kept < want || z != z) {  // (the same for every thread)
+            kept = want;
+            select_any<T, NT>(x, sp, kept, order_of(tau), sh, tid);
         }
     }
     return Part{m, z, s, shift};
@@ -388,6 +403,7 @@ __device__ __forceinline__ void in_order(const unsigned long long *keys, int n, 
         const int i = i0 + (tid >> 3);
         const unsigned long long key = i < n ? keys[i] : ~0ull;
         int rank = 0;
+#pragma unroll 4
         for (int j = tid & 7; j < n; j += 8) rank += keys[j] > key ? 1 : 0;
         rank += dpp_i<DPP_QUAD_XOR1>(rank);
         rank += dpp_i<DPP_QUAD_XOR2>(rank);
@@ -398,7 +414,7 @@ __device__ __forceinline__ void in_order(const unsigned long long *keys, int n, 
 
 // A workgroup per row.
 template <typename T, int NT, int MAXC>
-__global__ __launch_bounds__(NT) void logprobs_kernel(const T *__restrict__ logits, LogprobArgs a) {
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(MAXC >= 16 ? 4 : 1))) void logprobs_kernel(const T *__restrict__ logits, LogprobArgs a) {
     __shared__ Shared<NT> sh;
     const unsigned r = blockIdx.x;
     const int tid = threadIdx.x;
@@ -408,76 +424,71 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const T *__restrict__ logi
         return;
     }
     const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows);
-    const float x_tok = tok < a.V ? (float)x[tok] : 0.f;
+    const T x_tok = x[tok < a.V ? tok : 0];
     int kept = 0;
-    const Part p = scan_part<T, NT, MAXC>(x, a.V, 0, a.top, a.stats != nullptr, sh, tid, kept);
+    const Part p = scan_part<T, NT, MAXC>(x, a.V, a.top, a.stats != nullptr, sh, tid, kept, nullptr);
     const bool none = p.z == 0.f;  // nothing but -inf (a NaN makes z NaN)
     const float mm = none ? 0.f : p.m, l2 = log2f(p.z), lz = (l2 - p.shift) * LN2, H = none ? 0.f : (l2 - p.s / p.z) * LN2;
-    if (tid == 0) write_row(a, r, tok, x_tok, mm, lz, H, none);
+    if (tid == 0) write_row(a, r, tok, (float)x_tok, mm, lz, H, none);
     in_order<NT>(sh.key, kept, a.top, tid, [&](unsigned long long key, int k) {
         a.top_tokens[(int64_t)r * a.top + k] = index_of(key);
         a.top_logprobs[(int64_t)r * a.top + k] = none ? NEG_INF_F : (value_of(key) - mm) - lz;
     });
 }
 
-// A row in several parts (few rows, or more than the registers of a workgroup hold): a workgroup each leaves its maximum,
-// sums and largest keys, in order, in the workspace ...
-template <typename T, int NT, int MAXC>
-__global__ __launch_bounds__(NT) void logprobs_part_kernel(const T *__restrict__ logits, LogprobArgs a, int part_len,
-                                                           unsigned long long *__restrict__ work) {
-    __shared__ Shared<NT> sh;
+// A row in several parts, where it is more than the registers of a workgroup hold.  Each part's workgroup leaves its sums and
+// the maximum of every lane's elements in the workspace: two words, then PART_NT floats ...
+constexpr int PART_NT = 256, PART_MAXC = 20;
+constexpr int PART_WORDS = 2 + PART_NT / 2;
+template <typename T>
+__global__ __launch_bounds__(PART_NT) void logprobs_part_kernel(const T *__restrict__ logits, LogprobArgs a, int part_len,
+                                                                unsigned long long *__restrict__ work) {
+    __shared__ Shared<PART_NT> sh;
     const unsigned r = blockIdx.x;
     const int part = blockIdx.y, parts = gridDim.y, tid = threadIdx.x;
     if (a.tokens && a.tokens[r] < 0) return;
-    const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows);
     const int base = part * part_len;
+    const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows) + base;
     const int n = a.V - base < part_len ? a.V - base : part_len;
-    int kept = 0;
-    const Part p = scan_part<T, NT, MAXC>(x + base, n, base, a.top, a.stats != nullptr, sh, tid, kept);
-    unsigned long long *out = work + ((int64_t)r * parts + part) * (2 + a.top);
+    unsigned long long *out = work + ((int64_t)r * parts + part) * PART_WORDS;
+    int none = 0;
+    const Part p = scan_part<T, PART_NT, PART_MAXC>(x, n, 0, true, sh, tid, none, a.top > 0 ? reinterpret_cast<float *>(out + 2) : nullptr);
     if (tid == 0) {
         out[0] = ((unsigned long long)__float_as_uint(p.z) << 32) | __float_as_uint(p.m);
         out[1] = ((unsigned long long)__float_as_uint(p.shift) << 32) | __float_as_uint(p.s);
     }
-    in_order<NT>(sh.key, kept, a.top, tid, [&](unsigned long long key, int k) { out[2 + k] = key; });
-    for (int k = kept + tid; k < a.top; k += NT) out[2 + k] = 0;
 }
 
-// ... and a workgroup per row joins them: the sums are rescaled to the row's maximum, and the keys that can be among the
-// largest are put in order: those at or above every part's last key (its part alone has `top` of them) and at or above the
-// lowest of the parts' q-th keys (q = top / parts, rounded up: all parts together have).
-constexpr int JOIN_NT = 256;
+// ... and a workgroup per row joins the sums, rescaled to the row's maximum, and finds the alternatives: a threshold from the
+// lanes' maxima as scan_part takes it from its own, the lanes at or above it (hardly more than `top` of some thousand),
+// whose elements alone are read again, their candidates in order.  (Ordered lists from every part instead: 64 alternatives
+// of 64 rows of 250007 float32 in 38 us instead of NEW us.)
+constexpr int JOIN_NT = 1024;
 template <typename T>
-__global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restrict__ logits, LogprobArgs a, int parts,
+__global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restrict__ logits, LogprobArgs a, int part_len, int parts,
                                                                 const unsigned long long *__restrict__ work) {
-    __shared__ unsigned long long s_key[MAX_PARTS * MAX_TOP];
-    __shared__ unsigned long long s_floor;
-    __shared__ int s_n;
+    constexpr int N = VocabElem<T>::N, NW = JOIN_NT / 64, MAX_LANES = 512;
+    __shared__ Shared<JOIN_NT> sh;
+    __shared__ int s_lane[MAX_LANES];
+    __shared__ int s_lanes;
     const unsigned r = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int64_t tok = a.tokens ? a.tokens[r] : 0;
     if (tok < 0) {
         if (tid < 64) write_left_out(a, r, tid);
         return;
     }
     const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows);
-    const float x_tok = tok < a.V ? (float)x[tok] : 0.f;
-    const int each = 2 + a.top;
-    const unsigned long long *in = work + (int64_t)r * parts * each;
+    const T x_tok = x[tok < a.V ? tok : 0];
+    const unsigned long long *in = work + (int64_t)r * parts * PART_WORDS;
     // every wave forms the row's sums, lane by lane over the parts
     float m_p = NEG_INF_F, z_p = 0.f, s_p = 0.f, shift_p = 0.f;
-    unsigned long long last = 0, below = 0;  // (below: all ones less the part's q-th key)
     if (lane < parts) {
-        const unsigned long long zm = in[lane * each];
+        const unsigned long long zm = in[lane * PART_WORDS], hs = in[lane * PART_WORDS + 1];
         m_p = __uint_as_float((unsigned)zm);
         z_p = __uint_as_float((unsigned)(zm >> 32));
-        const unsigned long long hs = in[lane * each + 1];
         s_p = __uint_as_float((unsigned)hs);
         shift_p = __uint_as_float((unsigned)(hs >> 32));
-        if (a.top > 0) {
-            last = in[lane * each + 1 + a.top];
-            below = ~in[lane * each + 1 + (a.top + parts - 1) / parts];
-        }
     }
     const float m = wave_max(m_p), mm = m == NEG_INF_F ? 0.f : m;
     float z = 0.f, s = 0.f;
@@ -491,27 +502,88 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     s = wave_sum(s);
     const bool none = z == 0.f;
     const float l2 = log2f(z), lz = l2 * LN2, H = none ? 0.f : (l2 - s / z) * LN2;
-    if (tid == 0) write_row(a, r, tok, x_tok, mm, lz, H, none);
+    if (tid == 0) write_row(a, r, tok, (float)x_tok, mm, lz, H, none);
     if (a.top == 0) return;
-    last = wave_max_key(last);
-    below = ~wave_max_key(below);
-    if (tid == 0) {
-        s_floor = last > below ? last : below;
-        s_n = 0;
+
+    constexpr int U = 4;  // reads on their way together
+    const auto lane_max = [&](int l) { return l < parts * PART_NT ? reinterpret_cast<const float *>(in + (l / PART_NT) * PART_WORDS + 2)[l % PART_NT] : NEG_INF_F; };
+    const int all = parts * PART_NT;
+    float v[U], mine = NEG_INF_F;
+    for (int l0 = tid; l0 < all; l0 += U * JOIN_NT) {
+#pragma unroll
+        for (int u = 0; u < U; u++) v[u] = lane_max(l0 + u * JOIN_NT);
+#pragma unroll
+        for (int u = 0; u < U; u++) mine = max2_raw(mine, v[u]);
+    }
+    float tau = wave_max_raw(mine), rest = mine;
+    for (int q = (a.top + NW - 1) / NW; q > 1; q--) {
+        rest = rest == tau ? NEG_INF_F : rest;
+        tau = wave_max_raw(rest);
+    }
+    if (lane == 0) sh.tau[wave] = tau;
+    if (tid == 0) sh.n = s_lanes = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; w++) tau = sh.tau[w] < tau ? sh.tau[w] : tau;
+    for (int l0 = tid; l0 < all; l0 += U * JOIN_NT) {
+        if (all > U * JOIN_NT) {  // (more than the registers still hold)
+#pragma unroll
+            for (int u = 0; u < U; u++) v[u] = lane_max(l0 + u * JOIN_NT);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (v[u] >= tau && l0 + u * JOIN_NT < all) {
+                const int at = atomicAdd(&s_lanes, 1);
+                if (at < MAX_LANES) s_lane[at] = l0 + u * JOIN_NT;
+            }
     }
     __syncthreads();
-    const unsigned long long floor = s_floor;
-    for (int i0 = tid; i0 < parts * each; i0 += 8 * JOIN_NT) {  // (eight reads on their way; the parts' first two words are no keys)
-        unsigned long long key[8];
+    const int lanes = s_lanes;
+    bool fits = lanes <= MAX_LANES && z == z;
+    if (fits) {
+        const auto candidate = [&](float v, int i) {
+            if (v >= tau) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < Shared<JOIN_NT>::MAX_KEYS) sh.key[at] = key_of(v, i);
+            }
+        };
+        // an item is one chunk of a lane, its last item the scalar that the lane may hold besides
+        const int items = lanes * (PART_MAXC + 1);
+        for (int i0 = tid; i0 < items; i0 += 4 * JOIN_NT) {
+            vec16 v[4];
+            int at[4];
 #pragma unroll
-        for (int u = 0; u < 8; u++) key[u] = i0 + u * JOIN_NT < parts * each ? in[i0 + u * JOIN_NT] : 0;
+            for (int u = 0; u < 4; u++) {
+                at[u] = -1;
+                const int i = i0 + u * JOIN_NT;
+                if (i >= items) continue;
+                const int l = s_lane[i / (PART_MAXC + 1)], k = i % (PART_MAXC + 1), part = l / PART_NT, t = l % PART_NT;
+                const int base = part * part_len, n = a.V - base < part_len ? a.V - base : part_len;
+                const Span<T> sp(x + base, n);
+                if (k == PART_MAXC) {
+                    const int e = sp.edge(t);
+                    if (e >= 0) candidate((float)x[base + e], base + e);
+                } else if (t + k * PART_NT < sp.nvec) {
+                    at[u] = base + sp.head + (t + k * PART_NT) * N;
+                    v[u] = *reinterpret_cast<const vec16 *>(x + at[u]);
+                }
+            }
 #pragma unroll
-        for (int u = 0; u < 8; u++)
-            if (key[u] != 0 && key[u] >= floor && (i0 + u * JOIN_NT) % each >= 2) s_key[atomicAdd(&s_n, 1)] = key[u];
+            for (int u = 0; u < 4; u++)
+                if (at[u] >= 0) {
+                    const typename VocabElem<T>::vecT w = __builtin_bit_cast(typename VocabElem<T>::vecT, v[u]);
+#pragma unroll
+                    for (int k = 0; k < N; k++) candidate((float)w[k], at[u] + k);
+                }
+        }
     }
     __syncthreads();
-    const int n = s_n;
-    in_order<JOIN_NT>(s_key, n, a.top, tid, [&](unsigned long long key, int k) {
+    int n = sh.n;
+    if (!fits || n > Shared<JOIN_NT>::MAX_KEYS || n < a.top) {  // (the same for every thread)
+        n = a.top;
+        select_any<T, JOIN_NT>(x, Span<T>(x, a.V), n, order_of(tau), sh, tid);
+    }
+    in_order<JOIN_NT>(sh.key, n, a.top, tid, [&](unsigned long long key, int k) {
         a.top_tokens[(int64_t)r * a.top + k] = index_of(key);
         a.top_logprobs[(int64_t)r * a.top + k] = none ? NEG_INF_F : (value_of(key) - mm) - lz;
     });
@@ -523,41 +595,40 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
 struct Cut {
     int parts, len;
 };
-constexpr int MAX_CHUNKS = 512 * 20, PART_CHUNKS = 256 * 10;
+constexpr int MAX_CHUNKS = 512 * 20, PART_CHUNKS = PART_NT * PART_MAXC;
 inline Cut cut_of(int es, int64_t V) {
     const int64_t n = 16 / es, chunks = (V + n - 1) / n;
     if (chunks <= MAX_CHUNKS) return Cut{1, (int)V};
-    int64_t parts = (chunks + PART_CHUNKS - 1) / PART_CHUNKS;
-    if (parts > MAX_PARTS) parts = MAX_PARTS;
-    const int64_t len = (chunks + parts - 1) / parts * n;
+    const int64_t parts = (chunks + PART_CHUNKS - 1) / PART_CHUNKS, len = (chunks + parts - 1) / parts * n;
     return Cut{(int)((V + len - 1) / len), (int)len};
 }
 
 template <typename T, int NT, int MAXC>
-void launch_rows(const T *x, const LogprobArgs &a, const Cut &c, unsigned long long *work, hipStream_t s) {
-    if (c.parts == 1) hipLaunchKernelGGL((logprobs_kernel<T, NT, MAXC>), dim3((unsigned)a.rows), dim3(NT), 0, s, x, a);
-    else
-        hipLaunchKernelGGL((logprobs_part_kernel<T, NT, MAXC>), dim3((unsigned)a.rows, (unsigned)c.parts), dim3(NT), 0, s, x, a, c.len, work);
+void launch_rows(const T *x, const LogprobArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((logprobs_kernel<T, NT, MAXC>), dim3((unsigned)a.rows), dim3(NT), 0, s, x, a);
 }
 template <typename T>
 int launch_forward(const void *logits, const LogprobArgs &a, void *work, hipStream_t s) {
     const T *x = (const T *)logits;
     const Cut c = cut_of((int)sizeof(T), a.V);
     const int chunks = (c.len + VocabElem<T>::N - 1) / VocabElem<T>::N;
-    unsigned long long *w = (unsigned long long *)work;
-    // (every wave of a workgroup has to have elements: the alternatives' threshold is taken from all of them)
-    if (chunks <= 64 * 2) launch_rows<T, 64, 2>(x, a, c, w, s);
-    else if (chunks <= 64 * 8) launch_rows<T, 64, 8>(x, a, c, w, s);
-    else if (chunks <= 256 * 4) launch_rows<T, 256, 4>(x, a, c, w, s);
-    else if (chunks <= 256 * 10) launch_rows<T, 256, 10>(x, a, c, w, s);
-    else if (chunks <= 512 * 10 && a.rows < 512) launch_rows<T, 512, 10>(x, a, c, w, s);
-    else if (chunks <= 256 * 20) launch_rows<T, 256, 20>(x, a, c, w, s);
-    else launch_rows<T, 512, 20>(x, a, c, w, s);
-    PCFGNAT_HIP_CHECK(hipGetLastError());
     if (c.parts > 1) {
-        hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3((unsigned)a.rows), dim3(JOIN_NT), 0, s, x, a, c.parts, w);
+        unsigned long long *w = (unsigned long long *)work;
+        hipLaunchKernelGGL(logprobs_part_kernel<T>, dim3((unsigned)a.rows, (unsigned)c.parts), dim3(PART_NT), 0, s, x, a, c.len, w);
         PCFGNAT_HIP_CHECK(hipGetLastError());
+        hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3((unsigned)a.rows), dim3(JOIN_NT), 0, s, x, a, c.len, c.parts, w);
+        PCFGNAT_HIP_CHECK(hipGetLastError());
+        return PCFGNAT_OK;
     }
+    // (every wave of a workgroup has to have elements: the alternatives' threshold is taken from all of them)
+    if (chunks <= 64 * 2) launch_rows<T, 64, 2>(x, a, s);
+    else if (chunks <= 64 * 8) launch_rows<T, 64, 8>(x, a, s);
+    else if (chunks <= 256 * 4) launch_rows<T, 256, 4>(x, a, s);
+    else if (chunks <= 256 * 10) launch_rows<T, 256, 10>(x, a, s);
+    else if (chunks <= 512 * 10 && a.rows < 512) launch_rows<T, 512, 10>(x, a, s);
+    else if (chunks <= 256 * 20) launch_rows<T, 256, 20>(x, a, s);
+    else launch_rows<T, 512, 20>(x, a, s);
+    PCFGNAT_HIP_CHECK(hipGetLastError());
     return PCFGNAT_OK;
 }
 
@@ -598,10 +669,14 @@ __global__ __launch_bounds__(NT) void logprobs_grad_kernel(const T *__restrict__
     const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows) + base;
     const vec16_any *xv = reinterpret_cast<const vec16_any *>(x + sp.head);
     vec16 buf[MAXC];
+    const T edge = x[ei >= 0 ? ei : 0];
+    if (sp.nvec > 0) {  // (threads behind the last chunk read that one again: no branch around a load)
 #pragma unroll
-    for (int i = 0; i < MAXC; i++)
-        if (tid + i * NT < sp.nvec) buf[i] = __builtin_nontemporal_load(xv + tid + i * NT);
-    const float edge = ei >= 0 ? (float)x[ei] : 0.f;
+        for (int i = 0; i < MAXC; i++) buf[i] = __builtin_nontemporal_load(xv + (tid + i * NT < sp.nvec ? tid + i * NT : sp.nvec - 1));
+    } else {
+#pragma unroll
+        for (int i = 0; i < MAXC; i++) buf[i] = vec16{0u, 0u, 0u, 0u};
+    }
     const float m = a.stats[r], H = a.stats[2 * a.rows + r];
     const float gh = a.g_entropy ? a.g_entropy[r] : 0.f;
     for (int i = tid; i < NT * MAXC / 4; i += NT) s_hit[i] = 0;
@@ -631,24 +706,27 @@ __global__ __launch_bounds__(NT) void logprobs_grad_kernel(const T *__restrict__
         const float lp = (v - m) - lz;
         return -__builtin_amdgcn_exp2f(lp * LOG2E) * __builtin_fmaf(gh, fmaxf(lp, -1e30f), K);
     };
-    const auto arrivals = [&](float g, int at) {
-        for (int k = 0; k <= a.top; k++)
-            if (s_i[k] == at) g += s_g[k];
-        return g;
-    };
-    if (ei >= 0) dx[ei] = (T)arrivals(of(edge), ei);
+    if (ei >= 0) {
+        float g = of((float)edge);
+        for (int k = 0; k <= a.top; k++) g += s_i[k] == ei ? s_g[k] : 0.f;
+        dx[ei] = (T)g;
+    }
     const unsigned char *hit = reinterpret_cast<const unsigned char *>(s_hit);
 #pragma unroll
     for (int i = 0; i < MAXC; i++) {
         const int c = tid + i * NT;
+        float o[N];
+        VocabElem<T>::unpack(buf[i], o);
+#pragma unroll
+        for (int k = 0; k < N; k++) o[k] = of(o[k]);
         if (c < sp.nvec) {
-            float o[N];
-            VocabElem<T>::unpack(buf[i], o);
-#pragma unroll
-            for (int k = 0; k < N; k++) o[k] = of(o[k]);
             if (hit[c]) {
+#pragma unroll 1
+                for (int e = 0; e <= a.top; e++) {
+                    const int at = s_i[e] - (sp.head + c * N);
 #pragma unroll
-                for (int k = 0; k < N; k++) o[k] = arrivals(o[k], sp.head + c * N + k);
+                    for (int k = 0; k < N; k++) o[k] += at == k ? s_g[e] : 0.f;
+                }
             }
             __builtin_nontemporal_store(VocabElem<T>::pack(o), dv + c);
         }
@@ -685,7 +763,7 @@ using namespace pcfgnat;
 extern "C" size_t pcfgnat_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t V, int top) {
     if (!vocab_dtype_ok(dtype) || rows <= 0 || V < 1 || V > MAX_LOGPROB_VOCAB || top < 0) return 0;
     const Cut c = cut_of(vocab_elem_bytes(dtype), V);
-    return c.parts == 1 ? 0 : (size_t)rows * c.parts * (2 + top) * 8;
+    return c.parts == 1 ? 0 : (size_t)rows * c.parts * PART_WORDS * 8;
 }
 
 extern "C" int pcfgnat_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer,
