@@ -112,60 +112,94 @@ inline size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 inline size_t order_bytes(const Plan &p) { return align16((size_t)p.N * 4); }
 
 constexpr int SORT_NT = 1024, SORT_NW = SORT_NT / 64;
-constexpr int MAX_OWN = 1024;  // tokens of the vocabulary that one workgroup owns, at the most
+constexpr int MAX_OWN = 1024;   // tokens of the vocabulary that one workgroup owns, at the most
+constexpr int SORT_LIST = 256;  // tokens of its own that a wave remembers from the first look to the second
+constexpr int SORT_U = 4;       // groups of 64 positions whose reads are on their way together
 
 // Workgroup b of 2^block_bits owns the tokens b, b + 2^block_bits, ... of the vocabulary - spread, because vocabularies are
-// sorted by frequency: in strips the first workgroup would place half of all tokens (32768 tokens of 64000: 37 us in
-// strips) - and looks for them among all positions, each wave in its sixteenth: first how often each occurs
-// (and how many belong to the workgroups before this one, which is where its part of the order begins: no workgroup waits
-// for another), then each to its place, in ascending position.  The lanes that hold the same token are found by one ballot
-// for each bit of the token; the last of them moves the token's cursor on for all.  64 positions cost the same whether
-// they hold one token or 64.
+// sorted by frequency: in strips the first workgroup would place half of all tokens - and looks for them among all
+// positions, each wave in its sixteenth: first how often each occurs (and how many belong to the workgroups before this
+// one, which is where its part of the order begins: no workgroup waits for another), then each to its place, in ascending
+// position.  What bounds it is the look at every position, a dozen instructions for 64; the second look goes over the few
+// that the first has listed, or, where a wave has met more than its list holds (a common token), over all again.
+// The lanes that hold the same token are found by one ballot for each bit of the token; the last of them moves the token's
+// cursor on for all, so 64 positions cost the same whether they hold one token or 64.
 __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t *__restrict__ tokens, int64_t padding_idx, int N, int64_t V,
                                                                   int block_bits, int own_bits, int *__restrict__ count,
                                                                   int *__restrict__ counts, int *__restrict__ starts,
                                                                   int *__restrict__ order_pos, int *__restrict__ order_tok) {
-    __shared__ int s_at[SORT_NW][MAX_OWN];
+    extern __shared__ int s_at[];  // [SORT_NW][ids]: occurrences, then cursors
+    __shared__ unsigned s_list[SORT_NW][SORT_LIST];
     __shared__ int s_below[SORT_NW], s_wave[SORT_NW];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int block = (int)blockIdx.x, block_mask = (1 << block_bits) - 1;
     const int ids = (int)((V - block + block_mask) >> block_bits);
-    for (int i = lane; i < ids; i += 64) s_at[wave][i] = 0;
-    const int groups = (N + 63) / 64, each = (groups + SORT_NW - 1) / SORT_NW;
+    int *at_wave = s_at + wave * ids;
+    for (int i = lane; i < ids; i += 64) at_wave[i] = 0;
+    const int groups = (int)(((int64_t)N + 63) / 64), each = (groups + SORT_NW - 1) / SORT_NW;
     const int from = wave * each, to = from + each < groups ? from + each : groups;
-    const auto load = [&](int g) -> int64_t {
-        const int64_t at = (int64_t)g * 64 + lane;
-        return g < to && at < N ? tokens[at] : -1;
-    };
-    // the token of a lane among the workgroup's own; -1 where it belongs to one before, -2 where to neither
-    const auto local = [&](int64_t t) {
-        const bool real = t >= 0 && t < V && t != padding_idx;
-        const int owner = (int)t & block_mask;
-        return !real || owner > block ? -2 : owner < block ? -1 : (int)(t >> block_bits);
-    };
-    int below = 0;
-    unsigned long long found = 0;  // rounds of the first 64 that hold a token of this workgroup
-    constexpr int U = 8;
-    for (int g = from, round = 0; g < to; g += U, round++) {
-        int64_t t[U];
-        bool any = false;
+    // goes over the wave's positions, a round of SORT_U groups at a time: f(token, the lanes that hold a real one, group).  The next
+    // round's reads are ahead of what f stores, so that a wait for them (the hardware counts both in order) is none for the
+    // stores.  Masks of lanes are scalar: a group is a handful of vector instructions where it holds none of the own tokens.
+    const uint64_t *words = reinterpret_cast<const uint64_t *>(tokens);
+    const auto look = [&](auto f) {
+        uint64_t w[SORT_U], next[SORT_U];
+        const auto load = [&](uint64_t (&to_w)[SORT_U], int g) {
+            if (((int64_t)g + SORT_U) * 64 <= N) {
+                const uint64_t *at = words + (int64_t)g * 64;
 #pragma unroll
-        for (int u = 0; u < U; u++) t[u] = load(g + u);
+                for (int u = 0; u < SORT_U; u++) to_w[u] = at[u * 64 + lane];
+            } else {  // (the last position again behind the end)
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int id = local(t[u]);
-            below += __popcll(__ballot(id == -1));
-            if (id >= 0) atomicAdd(&s_at[wave][id], 1);
-            any |= id >= 0;
+                for (int u = 0; u < SORT_U; u++) {
+                    const int64_t at = ((int64_t)g + u) * 64 + lane;
+                    to_w[u] = words[at < N ? at : N - 1];
+                }
+            }
+        };
+        load(w, from);
+        for (int g = from; g < to; g += SORT_U) {
+            load(next, g + SORT_U);
+            if (g + SORT_U <= to && ((int64_t)g + SORT_U) * 64 <= N) {
+#pragma unroll
+                for (int u = 0; u < SORT_U; u++) f(w[u], __ballot(w[u] < (uint64_t)V) & __ballot(w[u] != (uint64_t)padding_idx), g + u);
+            } else {
+#pragma unroll
+                for (int u = 0; u < SORT_U; u++) {
+                    const int64_t left = g + u < to ? N - ((int64_t)g + u) * 64 : 0;
+                    const unsigned long long there = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+                    f(w[u], there & __ballot(w[u] < (uint64_t)V) & __ballot(w[u] != (uint64_t)padding_idx), g + u);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < SORT_U; u++) w[u] = next[u];
         }
-        if (round < 64 && __ballot(any)) found |= 1ull << round;
-    }
+    };
+    // appends the own tokens of a group to the wave's list (a ring)
+    const auto append = [&](uint64_t w, unsigned long long own, int g, int &listed) {
+        if ((own >> lane) & 1)
+            s_list[wave][(listed + __popcll(own & ((1ull << lane) - 1))) & (SORT_LIST - 1)] =
+                (unsigned)(w >> block_bits) << 22 | (unsigned)((g - from) * 64 + lane);
+        listed += __popcll(own);
+    };
+    int below = 0, listed = 0;
+    if (from < to)
+        look([&](uint64_t w, unsigned long long is, int g) {
+            const int owner = (int)w & block_mask;
+            below += __popcll(is & __ballot(owner < block));
+            const unsigned long long own = is & __ballot(owner == block);
+            if (own == 0) return;
+            if ((own >> lane) & 1) atomicAdd(&at_wave[w >> block_bits], 1);
+            append(w, own, g, listed);
+        });
     if (lane == 0) s_below[wave] = below;
     __syncthreads();
     // exclusive sums over (token, wave)
     int mine = 0;
-    if (tid < ids)
-        for (int w = 0; w < SORT_NW; w++) mine += s_at[w][tid];
+    if (tid < ids) {
+#pragma unroll
+        for (int w = 0; w < SORT_NW; w++) mine += s_at[w * ids + tid];
+    }
     int upto = mine;
     for (int d = 1; d < 64; d <<= 1) {
         const int v = __shfl_up(upto, d);
@@ -174,6 +208,7 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
     if (lane == 63) s_wave[wave] = upto;
     __syncthreads();
     int base = upto - mine, all_before = 0, all_own = 0;
+#pragma unroll
     for (int w = 0; w < SORT_NW; w++) {
         all_before += s_below[w];
         if (w < wave) base += s_wave[w];
@@ -182,9 +217,10 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
     base += all_before;
     if (tid < ids) {
         int at = base;
+#pragma unroll
         for (int w = 0; w < SORT_NW; w++) {
-            const int c = s_at[w][tid];
-            s_at[w][tid] = at;
+            const int c = s_at[w * ids + tid];
+            s_at[w * ids + tid] = at;
             at += c;
         }
         counts[((int64_t)tid << block_bits) + block] = mine;
@@ -192,31 +228,44 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
     }
     if (block == block_mask && tid == 0) *count = all_before + all_own;
     __syncthreads();
-    for (int g = from, round = 0; g < to; g += U, round++) {
-        if (round < 64 && !((found >> round) & 1)) continue;
-        int64_t t[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) t[u] = load(g + u);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int id = local(t[u]);
-            unsigned long long same = __ballot(id >= 0);
-            if (same == 0) continue;
+    // `n` listed tokens, from the first-th on, to their places
+    const auto place = [&](int first, int n) {
+        const bool own = lane < n;
+        const unsigned e = s_list[wave][(first + (own ? lane : 0)) & (SORT_LIST - 1)];
+        const int id = (int)(e >> 22);
+        unsigned long long same = __ballot(own);
+        if (same & __ballot(id != __builtin_amdgcn_readfirstlane(id)))  // (one token alone is common: a run's)
             for (int bit = 0; bit < own_bits; bit++) {
-                const unsigned long long set = __ballot((id >> bit) & 1);
-                same &= (id >> bit) & 1 ? set : ~set;
+                const bool one = (id >> bit) & 1;
+                const unsigned long long set = __ballot(one);
+                same &= one ? set : ~set;
             }
-            if (id >= 0) {
-                // (the cursor of this wave alone; read by all lanes of the token before the last of them writes it)
-                const int at = __hip_atomic_load(&s_at[wave][id], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                const int rank = __popcll(same & ((1ull << lane) - 1)), all = __popcll(same);
-                if (rank == all - 1) __hip_atomic_store(&s_at[wave][id], at + all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                order_pos[at + rank] = (g + u) * 64 + lane;
-                order_tok[at + rank] = (int)t[u];
-            }
-            __builtin_amdgcn_wave_barrier();
+        if (own) {
+            // (the cursor of this wave alone; read by all lanes of the token before the last of them writes it)
+            const int at = __hip_atomic_load(&at_wave[id], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            const int rank = __popcll(same & ((1ull << lane) - 1)), all = __popcll(same);
+            if (rank == all - 1) __hip_atomic_store(&at_wave[id], at + all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            order_pos[at + rank] = from * 64 + (int)(e & 0x3FFFFF);
+            order_tok[at + rank] = (id << block_bits) + block;
         }
+        __builtin_amdgcn_wave_barrier();
+    };
+    int placed = 0;
+    if (listed > SORT_LIST) {  // the list was overwritten: once more, placing 64 whenever there are
+        listed = 0;
+        look([&](uint64_t w, unsigned long long is, int g) {
+            const unsigned long long own = is & __ballot(((int)w & block_mask) == block);
+            if (own == 0) return;
+            append(w, own, g, listed);
+            if (listed - placed >= 64) {
+                __builtin_amdgcn_wave_barrier();
+                place(placed, 64);
+                placed += 64;
+            }
+        });
     }
+    __builtin_amdgcn_wave_barrier();
+    for (; placed < listed; placed += 64) place(placed, listed - placed < 64 ? listed - placed : 64);
 }
 
 // A wave sums one piece of the order over a tile of 64 chunks of columns, 8 rows of g on their way at a time.  Runs that begin
@@ -236,9 +285,14 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const T *__restrict_
     if (p >= pieces) {
         const vec16 zero = {0u, 0u, 0u, 0u};
         const int64_t v0 = (task - pieces * tiles) * ZERO_ROWS;
-        for (int64_t v = v0; v < v0 + ZERO_ROWS && v < V; v++)
-            if (counts[v] == 0)
-                for (int64_t c = (int64_t)lane * E; c < D; c += 64 * E) store_columns(dweight + v * D, c, D, zero);
+        const bool unused = lane < ZERO_ROWS && v0 + lane < V && counts[v0 + lane < V ? v0 + lane : 0] == 0;
+        for (unsigned long long rows = __ballot(unused); rows; rows &= rows - 1) {
+            T *row = dweight + (v0 + __builtin_ctzll(rows)) * D;
+            if (NARROW) store_columns(row, 0, D, zero);
+            else
+                for (int64_t c = (int64_t)lane * E; c < D; c += 64 * E)
+                    __builtin_nontemporal_store(zero, reinterpret_cast<vec16_any *>(row + (c + E <= D ? c : D - E)));
+        }
         return;
     }
     const int total = *count;
@@ -369,13 +423,15 @@ int backward(const void *g, int64_t gstride, const int64_t *tokens, float scale,
     int *count = (int *)w, *order_pos = (int *)(w + 16), *order_tok = (int *)(w + 16 + order_bytes(p));
     int *counts = (int *)(w + 16 + 2 * order_bytes(p)), *starts = (int *)((char *)counts + align16((size_t)V * 4));
     float *cut = (float *)((char *)starts + align16((size_t)V * 4));
-    // 256 workgroups, fewer for a small vocabulary (at least 16 tokens each), more for one beyond 256 * MAX_OWN
+    // 256 workgroups, fewer for a smaller vocabulary, more for one beyond 256 * MAX_OWN
     int block_bits = 0, own_bits = 0;
-    while (block_bits < 8 && (16 << (block_bits + 1)) <= V) block_bits++;
+    while (block_bits < 8 && ((int64_t)2 << block_bits) <= V) block_bits++;
     while (((V - 1) >> block_bits) + 1 > MAX_OWN) block_bits++;
     while (((int64_t)1 << own_bits) < ((V - 1) >> block_bits) + 1) own_bits++;
-    hipLaunchKernelGGL(embedding_order_kernel, dim3(1u << block_bits), dim3(SORT_NT), 0, s, tokens, padding_idx, (int)N, V, block_bits, own_bits,
-                       count, counts, starts, order_pos, order_tok);
+    const size_t lds = (size_t)SORT_NW * (((V - 1) >> block_bits) + 1) * 4;
+    PCFGNAT_DYNAMIC_LDS(embedding_order_kernel, SORT_NW * MAX_OWN * 4);
+    hipLaunchKernelGGL(embedding_order_kernel, dim3(1u << block_bits), dim3(SORT_NT), lds, s, tokens, padding_idx, (int)N, V, block_bits,
+                       own_bits, count, counts, starts, order_pos, order_tok);
     PCFGNAT_HIP_CHECK(hipGetLastError());
     if (D < VocabElem<T>::N)
         hipLaunchKernelGGL((embedding_sum_kernel<T, true>), dim3((unsigned)sum_blocks), dim3(256), 0, s, (const T *)g, gstride, scale,
@@ -393,7 +449,7 @@ int backward(const void *g, int64_t gstride, const int64_t *tokens, float scale,
     return PCFGNAT_OK;
 }
 
-constexpr int64_t MAX_TOKENS = 2147483647 - 4096;  // positions are kept in 32 bits
+constexpr int64_t MAX_TOKENS = (int64_t)SORT_NW << 22;  // (a list entry keeps 22 bits of a position in its wave's sixteenth)
 constexpr int64_t MAX_VOCAB = 1 << 26;
 constexpr int64_t MAX_DIM = 1 << 20;
 

@@ -481,6 +481,17 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows);
     const T x_tok = x[tok < a.V ? tok : 0];
     const unsigned long long *in = work + (int64_t)r * parts * PART_WORDS;
+    // the lanes' maxima: U a thread on their way from here on, more than that are read again
+    constexpr int U = 4;
+    const int all = a.top > 0 ? parts * PART_NT : 0;
+    const auto lane_max = [&](int l) { return reinterpret_cast<const float *>(in + (l / PART_NT) * PART_WORDS + 2)[l % PART_NT]; };
+    float v[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int l = tid + u * JOIN_NT;
+        v[u] = lane_max(l < all ? l : 0);  // (without alternatives nobody has written it and nobody looks at it)
+        if (l >= all) v[u] = NEG_INF_F;
+    }
     // every wave forms the row's sums, lane by lane over the parts
     float m_p = NEG_INF_F, z_p = 0.f, s_p = 0.f, shift_p = 0.f;
     if (lane < parts) {
@@ -505,16 +516,10 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     if (tid == 0) write_row(a, r, tok, (float)x_tok, mm, lz, H, none);
     if (a.top == 0) return;
 
-    constexpr int U = 4;  // reads on their way together
-    const auto lane_max = [&](int l) { return l < parts * PART_NT ? reinterpret_cast<const float *>(in + (l / PART_NT) * PART_WORDS + 2)[l % PART_NT] : NEG_INF_F; };
-    const int all = parts * PART_NT;
-    float v[U], mine = NEG_INF_F;
-    for (int l0 = tid; l0 < all; l0 += U * JOIN_NT) {
+    float mine = NEG_INF_F;
 #pragma unroll
-        for (int u = 0; u < U; u++) v[u] = lane_max(l0 + u * JOIN_NT);
-#pragma unroll
-        for (int u = 0; u < U; u++) mine = max2_raw(mine, v[u]);
-    }
+    for (int u = 0; u < U; u++) mine = max2_raw(mine, v[u]);
+    for (int l0 = tid + U * JOIN_NT; l0 < all; l0 += JOIN_NT) mine = max2_raw(mine, lane_max(l0));
     float tau = wave_max_raw(mine), rest = mine;
     for (int q = (a.top + NW - 1) / NW; q > 1; q--) {
         rest = rest == tau ? NEG_INF_F : rest;
@@ -525,18 +530,16 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NW; w++) tau = sh.tau[w] < tau ? sh.tau[w] : tau;
-    for (int l0 = tid; l0 < all; l0 += U * JOIN_NT) {
-        if (all > U * JOIN_NT) {  // (more than the registers still hold)
-#pragma unroll
-            for (int u = 0; u < U; u++) v[u] = lane_max(l0 + u * JOIN_NT);
+    const auto list = [&](float max, int l) {
+        if (max >= tau) {
+            const int at = atomicAdd(&s_lanes, 1);
+            if (at < MAX_LANES) s_lane[at] = l;
         }
+    };
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            if (v[u] >= tau && l0 + u * JOIN_NT < all) {
-                const int at = atomicAdd(&s_lanes, 1);
-                if (at < MAX_LANES) s_lane[at] = l0 + u * JOIN_NT;
-            }
-    }
+    for (int u = 0; u < U; u++)
+        if (tid + u * JOIN_NT < all) list(v[u], tid + u * JOIN_NT);
+    for (int l0 = tid + U * JOIN_NT; l0 < all; l0 += JOIN_NT) list(lane_max(l0), l0);
     __syncthreads();
     const int lanes = s_lanes;
     bool fits = lanes <= MAX_LANES && z == z;
