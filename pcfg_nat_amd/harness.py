@@ -49,15 +49,22 @@ def compute_pcfg_loss(outputs, output_masks, targets, target_masks, links, ops=_
 
 
 def glat_alignment(word_ins_out, tgt_tokens, prev_output_tokens, links, context_p, pad=PAD, ops=_default_ops,
-                   generator=None, noise_device=None, single_call=False, glance_strategy="number-random"):
+                   generator=None, noise_device=None, single_call=False, glance_strategy="number-random", embed=None):
     """GLAT glancing (nat_pcfg_loss.py:193-269): best-tree alignment of target tokens to graph nodes, then a random
     subset of the aligned nodes is revealed, chosen by the criterion's ``glance_strategy``: ``"number-random"`` (every
     shipped script; :235-242), ``"cmlm"`` (:244-251) or ``None`` (:231-233).  RNG order as in the reference: ``randn``
     (not for ``None``), ``rand`` over the batch (``cmlm`` only), ``rand`` over the nodes.  The reference draws on the
     tokens' device; ``noise_device`` (e.g. "cpu") draws elsewhere and moves the numbers, which makes a run reproducible
-    across devices.  ``single_call``: the same pass as one native call (``ops.pcfg_glat_step``)."""
+    across devices.  ``single_call``: the same pass as one native call (``ops.pcfg_glat_step``).  ``embed``: a pair (embedding
+    weight [vocab, dim], scale); the result then also holds ``decoder_input`` [bsz, prelen, dim], the scaled embeddings of
+    the glanced tokens, which the decoder takes next (differentiable in the weight, nothing arrives at ``pad``'s row)."""
     if glance_strategy not in ("number-random", "cmlm", None):
         raise RuntimeError("glat_alignment: unknown glance strategy %r" % (glance_strategy,))
+    if embed is not None:
+        out = glat_alignment(word_ins_out, tgt_tokens, prev_output_tokens, links, context_p, pad, ops, generator, noise_device, single_call,
+                             glance_strategy)
+        out["decoder_input"] = ops.token_embedding(embed[0], out["glat_prev_output_tokens"], scale=embed[1], padding_idx=pad)
+        return out
     if single_call:
         return ops.pcfg_glat_step(word_ins_out, tgt_tokens, prev_output_tokens, links, context_p, pad, generator=generator,
                                   noise_device=noise_device, glance_strategy=glance_strategy)
@@ -124,10 +131,21 @@ def viterbi_decode(unreduced_logits, unreduced_tokens, links, output_length, lef
     return tokens.to(device=pred_length.device), pred_length
 
 
-def decode_from_logits(logits, links, output_length, left_tree_mask, pad=PAD, beta=1.0, ops=_default_ops, single_call=False):
+def decode_from_logits(logits, links, output_length, left_tree_mask, pad=PAD, beta=1.0, ops=_default_ops, single_call=False,
+                       alternatives=0):
     """The decode from the vocabulary logits, as the model runs it (glat_decomposed_with_link_two_hands_tri_pcfg.py:414-416,
     483-502): ``log_softmax`` and ``max`` over the vocabulary, then ``viterbi_decode``.  ``single_call``: both enqueued by
-    one native call (``ops.pcfg_viterbi_decode_logits``).  Returns (tokens float32 [B,maxlen], pred_length [B])."""
+    one native call (``ops.pcfg_viterbi_decode_logits``).  Returns (tokens float32 [B,maxlen], pred_length [B]).
+
+    ``alternatives`` > 0: the same read of the logits also gives every graph node's that many most probable tokens and the
+    entropy of its distribution (``ops.token_logprobs``, whose first alternative is the front-end's token), for confidences,
+    rescoring or n-best lists; returns (tokens, pred_length, ``TokenLogprobs`` with ``entropy`` [B,L] and ``top_*``
+    [B,L,alternatives])."""
+    if alternatives > 0:
+        nodes = ops.token_logprobs(logits, top=alternatives, entropy=True)
+        tokens, pred_length = viterbi_decode(nodes.top_logprobs[..., 0].contiguous(), nodes.top_tokens[..., 0].contiguous(), links,
+                                             output_length, left_tree_mask, pad, beta, ops=ops, single_call=True)
+        return tokens, pred_length, nodes
     if single_call:
         return ops.pcfg_viterbi_decode_logits(logits, links, output_length.long(), left_tree_mask, pad, beta)
     ob, tok = ops.logsoftmax_max(logits)

@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from pcfg_nat_amd import _lib, custom_ops as ops
+from pcfg_nat_amd import _lib, custom_ops as ops, harness, synth
 
 U = 2.0 ** -24
 TYPES = [torch.float16, torch.bfloat16, torch.float32]
@@ -492,6 +492,224 @@ def test_tied_weight_gradient_from_both_ends(dtype):
     mass.index_add_(0, tokens.cpu().reshape(-1), (dl @ wa) * 2.0)
     err = (weight.grad.double().cpu() - w.grad).abs()
     assert not (err > (4 * half_step(dtype) + 800 * U) * mass + 8 * SMALL[dtype]).any()
+
+
+@gpu
+@pytest.mark.parametrize("single_call", [False, True])
+def test_glancing_step_with_its_embeddings(single_call):
+    """The GLAT step with ``embed``: the tokens as without it, and the embeddings that the decoder takes next."""
+    batch = synth.config1()
+    B, L, V = batch["logits"].shape
+    prev = torch.full((B, L), 3, dtype=torch.int64)
+    prev[1, 24:] = synth.PAD
+    weight = torch.randn((V, 16), generator=torch.Generator().manual_seed(1)).to(DEV).requires_grad_(True)
+    args = (batch["targets"].to(DEV), prev.to(DEV), batch["links"].to(DEV), 0.5)
+    outs = []
+    for embed in (None, (weight, 4.0)):
+        outs.append(harness.glat_alignment(batch["logits"].clone().to(DEV), *args, generator=torch.Generator().manual_seed(7),
+                                           noise_device="cpu", single_call=single_call, embed=embed))
+    for key, value in outs[0].items():
+        assert torch.equal(outs[1][key], value)
+    glanced = outs[1]["glat_prev_output_tokens"]
+    up = torch.randn((B, L, 16), generator=torch.Generator().manual_seed(2)).to(DEV)
+    grad, = torch.autograd.grad(outs[1]["decoder_input"], weight, up)
+    check_embedding(weight, glanced, 4.0, synth.PAD, outs[1]["decoder_input"], up, grad)
+    assert (grad[synth.PAD] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("alternatives", [1, 6])
+def test_decode_with_alternatives(alternatives):
+    """The decode whose front-end also gives every node's alternatives: tokens and lengths as by the Viterbi decode over the
+    first alternatives, the same tokens as the model's own front-end finds, the alternatives those of the formulas."""
+    logits, links, ol, mask = (t.to(DEV) for t in _decode_case())
+    tokens, length, nodes = harness.decode_from_logits(logits, links, ol, mask, alternatives=alternatives)
+    best, idx = ops.logsoftmax_max(logits)
+    assert torch.equal(nodes.top_tokens[..., 0], idx) and (nodes.top_logprobs[..., 0] - best).abs().max() <= 2 * U * 240
+    want_tokens, want_length = harness.viterbi_decode(nodes.top_logprobs[..., 0].contiguous(), idx, links, ol, mask, single_call=True)
+    assert torch.equal(tokens, want_tokens) and torch.equal(length, want_length)
+    rows = logits.shape[0] * logits.shape[1]
+    check_logprobs(logits.reshape(rows, -1), None, alternatives, [None, nodes.entropy.reshape(rows)] + [t.reshape(rows, alternatives) for t in nodes[2:]])
+
+
+def _decode_case():
+    batch = synth.decode_batch([8, 5, 7], seed=3, V=700)
+    mask, _, _ = synth.support_masks(batch["logits"].shape[1], 1)
+    return batch["logits"], batch["links"], batch["output_length"], mask
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# streams, graphs, far offsets, the C-ABI
+# ------------------------------------------------------------------------------------------------------------------
+def _step(logits, tokens, weight, words, ups):
+    """A forward and backward of both operators; all results."""
+    got = ops.token_logprobs(logits, tokens, top=3, entropy=True)
+    dx, = torch.autograd.grad([got.logprobs, got.entropy, got.top_logprobs], logits, ups[:3])
+    out = ops.token_embedding(weight, words, scale=2.0, padding_idx=1)
+    dw, = torch.autograd.grad(out, weight, ups[3])
+    return [t.detach() for t in got] + [dx, out.detach(), dw]
+
+
+def _step_inputs(seed, V, rows=37):
+    gen = torch.Generator().manual_seed(seed)
+    logits = torch.randn((rows, V), generator=gen).half().to(DEV).requires_grad_(True)
+    tokens = torch.randint(-1, V, (rows,), generator=gen).to(DEV)
+    weight = torch.randn((500, 24), generator=gen).half().to(DEV).requires_grad_(True)
+    words = torch.where(torch.rand((300,), generator=gen) < 0.5, torch.tensor(3), torch.randint(0, 500, (300,), generator=gen)).to(DEV)
+    ups = [torch.randn(s, generator=gen).to(DEV) for s in ((rows,), (rows,), (rows, 3))] + [torch.randn((300, 24), generator=gen).half().to(DEV)]
+    return logits, tokens, weight, words, ups
+
+
+@gpu
+@pytest.mark.parametrize("V", [1001, 90001])
+def test_on_another_stream_and_from_threads(V):
+    """The same results, bit for bit, on a stream of its own behind work that the inputs wait for, and from two threads on two
+    streams at once."""
+    import threading
+    args = [_step_inputs(s, V) for s in (1, 2)]
+    want = [_step(*a) for a in args]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    source = args[0][0].detach().clone()
+    late = torch.zeros_like(source)
+    with torch.cuda.stream(side):
+        big = torch.ones((4096, 4096), device=DEV)
+        for _ in range(4):
+            big = big @ big * 1e-4
+        late.copy_(source)
+        got = _step(late.requires_grad_(True), *args[0][1:])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    results, errors = [[], []], []
+
+    def work(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    results[k].append(_step(*args[k]))
+            stream.synchronize()
+        except Exception as e:  # (shown by the assertion below)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for k in range(2):
+        for r in results[k]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[k]))
+
+
+@gpu
+@pytest.mark.parametrize("V", [1001, 90001])
+def test_captured_into_graphs(V):
+    """Forward and backward of both operators captured, two graphs out of one memory pool: replayed in turn with new inputs in
+    place and eager work between, every replay the eager results bit for bit."""
+    sets = [_step_inputs(s, V) for s in (3, 4)]
+    fresh = [_step_inputs(s, V) for s in (5, 6, 7)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for a in sets:
+            _step(*a)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for a in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=graphs[0].pool() if graphs else None):
+            outs.append(_step(*a))
+        graphs.append(g)
+    for turn, new in enumerate(fresh):
+        for k in range(2):
+            with torch.no_grad():
+                for into, value in zip(sets[k][:4], new[:4]):
+                    into.copy_(value)
+                for into, value in zip(sets[k][4], new[4]):
+                    into.copy_(value)
+            graphs[k].replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in outs[k]]
+            want = _step(*new)
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(got, want)), (turn, k)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^32 bytes and 2^31 elements of logits, of their gradient and of a weight: the last rows."""
+    gen = torch.Generator().manual_seed(8)
+    rows, V = 54000, 40000
+    assert rows * V > 2 ** 31
+    logits = torch.zeros((rows, V), dtype=torch.float16, device=DEV)
+    tail = (torch.randn((3, V), generator=gen) * 2).half().to(DEV)
+    logits[-3:] = tail
+    tokens = torch.full((rows,), -1, dtype=torch.int64, device=DEV)
+    tokens[-3:] = torch.tensor([0, V - 1, 77], device=DEV)
+    leaf = logits.requires_grad_(True)
+    got = ops.token_logprobs(leaf, tokens, top=4, entropy=True)
+    ups = [torch.randn(t.shape, generator=gen).to(DEV) for t in got[:3]]
+    grad, = torch.autograd.grad(got[:3], leaf, ups)
+    assert (grad[:3] == 0).all() and (grad[rows // 2] == 0).all()
+    check_logprobs(tail, tokens[-3:], 4, [t[-3:] for t in got], (grad[-3:], *[u[-3:] for u in ups]))
+    del leaf, logits, grad, got
+    torch.cuda.empty_cache()
+    V, D = 1100000, 2048
+    assert V * D > 2 ** 31
+    weight = torch.zeros((V, D), dtype=torch.float16, device=DEV)
+    weight[-2:] = torch.randn((2, D), generator=gen).half().to(DEV)
+    words = torch.tensor([V - 1, 0, V - 2, V - 1], device=DEV)
+    leaf = weight.requires_grad_(True)
+    out = ops.token_embedding(leaf, words, scale=3.0)
+    up = torch.randn((4, D), generator=gen).half().to(DEV)
+    grad, = torch.autograd.grad(out, leaf, up)
+    short = torch.cat([weight.detach()[:1], weight.detach()[-2:]])
+    check_embedding(short, torch.tensor([2, 0, 1, 2]), 3.0, None, out, up, torch.cat([grad[:1], grad[-2:]]))
+    assert not grad[1:-2].any()
+    del leaf, weight, grad, out
+    torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_c_abi_with_results_at_any_element(dtype):
+    """The entry points called directly, their results one element behind an aligned address; what lies around them stays."""
+    lib = _lib.load()
+    gen = torch.Generator().manual_seed(12)
+    code = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}[dtype]
+    stream = torch.cuda.current_stream().cuda_stream
+    rows, V = 5, 3001
+    x = torch.randn((rows, V), generator=gen).to(dtype).to(DEV)
+    tokens = some_tokens(rows, V, gen)
+    f = lambda *shape: torch.full(shape, 7.0, device=DEV)  # noqa: E731
+    lp, h, tl, stats = f(rows), f(rows), f(rows, 2), f(3, rows)
+    tt = torch.zeros((rows, 2), dtype=torch.int64, device=DEV)
+    _lib.check(lib.pcfgnat_token_logprobs(x.data_ptr(), code, 1, rows, 0, V, tokens.data_ptr(), lp.data_ptr(), h.data_ptr(), 2, tl.data_ptr(),
+                                          tt.data_ptr(), stats.data_ptr(), None, V, stream), lib)
+    guard = torch.full((rows * V + 2,), 7.0, dtype=dtype, device=DEV)
+    ups = [torch.randn(s, generator=gen).to(DEV) for s in ((rows,), (rows,), (rows, 2))]
+    _lib.check(lib.pcfgnat_token_logprobs_backward(x.data_ptr(), code, 1, rows, 0, V, tokens.data_ptr(), tt.data_ptr(), 2, stats.data_ptr(),
+                                                   ups[0].data_ptr(), ups[1].data_ptr(), ups[2].data_ptr(), guard[1:].data_ptr(), V, stream), lib)
+    assert guard[0] == 7 and guard[-1] == 7
+    check_logprobs(x, tokens, 2, (lp, h, tl, tt), (guard[1:-1].view(rows, V), *ups))
+    vocab, D, N = 40, 29, 64
+    weight = torch.randn((vocab, D), generator=gen).to(dtype).to(DEV)
+    words = torch.randint(0, vocab // 2, (N,), generator=gen).to(DEV)
+    out = torch.full((N * D + 2,), 7.0, dtype=dtype, device=DEV)
+    _lib.check(lib.pcfgnat_token_embedding(weight.data_ptr(), code, D, words.data_ptr(), 2.0, out[1:].data_ptr(), N, vocab, D, stream), lib)
+    dw = torch.full((vocab * D + 2,), 7.0, dtype=dtype, device=DEV)
+    up = torch.randn((N, D), generator=gen).to(dtype).to(DEV)
+    need = lib.pcfgnat_token_embedding_backward_workspace_bytes(N, vocab, D)
+    work = torch.full((need + 16,), 85, dtype=torch.uint8, device=DEV)
+    _lib.check(lib.pcfgnat_token_embedding_backward(up.data_ptr(), code, D, words.data_ptr(), 2.0, -1, dw[1:].data_ptr(), work.data_ptr(), N, vocab,
+                                                    D, stream), lib)
+    for t in (out, dw):
+        assert t[0] == 7 and t[-1] == 7
+    assert (work[need:] == 85).all()
+    check_embedding(weight, words, 2.0, None, out[1:-1].view(N, D), up, dw[1:-1].view(vocab, D))
 
 
 # ------------------------------------------------------------------------------------------------------------------
