@@ -480,7 +480,7 @@ int pcfgnat_token_embedding(const void *weight, int dtype, int64_t weight_stride
  * is written.  grad_out rows are grad_stride elements apart.  padding_idx (negative: none) and tokens outside [0, V) have no
  * gradient.  workspace: pcfgnat_token_embedding_backward_workspace_bytes bytes, 16-byte aligned.
  */
-size_t pcfgnat_token_embedding_backward_workspace_bytes(int64_t N, int64_t V, int64_t D);
+size_t pcfgnat_token_embedding_backward_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D);
 int pcfgnat_token_embedding_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, float scale,
                                      int64_t padding_idx, void *grad_weight, void *workspace, int64_t N, int64_t V, int64_t D,
                                      void *stream);

@@ -1,13 +1,19 @@
 // Host side of the operators on the two ends of the vocabulary: token_logprobs and token_embedding, each with its autograd
-// node.  Checks, allocation and the call into the C-ABI, like the training operators of torch_ext.cpp; without a gradient to
-// come the node is left out, which is most of the host's time on a single token.
+// node.  Checks, allocation and the call into the C-ABI, like the training operators of torch_ext.cpp.  On small batches the
+// host's time is the operator's: a node is made only where a gradient is to come, and made by hand (the general
+// torch::autograd::Function costs some microseconds more a pass in maps of attributes and outputs).
 #include "torch_ext.h"
+
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 #include <cmath>
 
 namespace {
 
-using torch::autograd::AutogradContext;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 int vocab_dtype(const char *who, const at::Tensor &t) {
@@ -21,6 +27,10 @@ int vocab_dtype(const char *who, const at::Tensor &t) {
 
 void no_second_derivative(const char *who) {
     TORCH_CHECK(!at::GradMode::is_enabled(), who, ": the gradient is not differentiable again (create_graph is not supported)");
+}
+
+void no_tangent(const char *who, const at::Tensor &t) {
+    TORCH_CHECK(!t._fw_grad(0).defined(), who, ": no forward-mode derivative");
 }
 
 // A gradient as the kernels read it: float32, contiguous; null where nothing arrived.
@@ -120,41 +130,30 @@ LogprobOutputs logprobs_forward(const Rows &r, at::IntArrayRef shape, const at::
     return o;
 }
 
-struct TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
-    // returns what was asked for, in the order log-probabilities, entropy, top log-probabilities, top tokens
-    static variable_list forward(AutogradContext *ctx, at::Tensor logits, at::Tensor tokens, int64_t top, bool entropy) {
-        const c10::DeviceGuard guard(logits.device());
-        const Rows r = rows_of(logits);
-        const at::IntArrayRef shape = logits.sizes().slice(0, logits.dim() - 1);
-        const LogprobOutputs o = logprobs_forward(r, shape, tokens, top, entropy, true);
-        ctx->set_materialize_grads(false);
-        variable_list out;
-        if (o.logprobs.defined()) out.push_back(o.logprobs);
-        if (o.entropy.defined()) out.push_back(o.entropy);
-        if (top > 0) {
-            out.push_back(o.top_logprobs);
-            out.push_back(o.top_tokens);
-            ctx->mark_non_differentiable({o.top_tokens});
-        }
-        ctx->save_for_backward({logits, tokens, o.stats, o.top_tokens});
-        ctx->saved_data["top"] = top;
-        ctx->saved_data["entropy"] = entropy;
-        return out;
-    }
+struct TokenLogprobsBackward : public Node {
+    SavedVariable logits_, tokens_, stats_, top_tokens_;
+    int64_t top = 0;
+    bool has_logprobs = false, has_entropy = false;
 
-    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    std::string name() const override { return "TokenLogprobsBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        logits_.reset_data();
+        tokens_.reset_data();
+        stats_.reset_data();
+        top_tokens_.reset_data();
+    }
+    variable_list apply(variable_list &&grads) override {
         const char *who = "token_logprobs";
         no_second_derivative(who);
-        const auto saved = ctx->get_saved_variables();
-        const at::Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2], &top_tokens = saved[3];
-        const int64_t top = ctx->saved_data["top"].toInt();
+        std::lock_guard<std::mutex> lock(mutex_);
         size_t at = 0;
         at::Tensor g_lp, g_h, g_top, k0, k1, k2;
-        if (tokens.defined()) g_lp = grads[at++];
-        if (ctx->saved_data["entropy"].toBool()) g_h = grads[at++];
+        if (has_logprobs) g_lp = grads[at++];
+        if (has_entropy) g_h = grads[at++];
         if (top > 0) g_top = grads[at++];
-        variable_list none(4);
-        if (!g_lp.defined() && !g_h.defined() && !g_top.defined()) return none;
+        if (!task_should_compute_output(0) || (!g_lp.defined() && !g_h.defined() && !g_top.defined())) return {at::Tensor()};
+        const at::Tensor logits = logits_.unpack(), tokens = tokens_.unpack(), stats = stats_.unpack(), top_tokens = top_tokens_.unpack();
         const c10::DeviceGuard guard(logits.device());
         const Rows r = rows_of(logits);
         at::Tensor grad = at::empty(logits.sizes(), logits.options().requires_grad(false), at::MemoryFormat::Contiguous);
@@ -163,8 +162,7 @@ struct TokenLogprobsFn : public torch::autograd::Function<TokenLogprobsFn> {
                                                  top > 0 ? top_tokens.data_ptr<int64_t>() : nullptr, (int)top, stats.data_ptr<float>(),
                                                  arrived(g_lp, k0), arrived(g_h, k1), arrived(g_top, k2), grad.data_ptr(), r.V,
                                                  stream_of(logits)));
-        none[0] = grad;
-        return none;
+        return {grad};
     }
 };
 
@@ -173,21 +171,27 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
     at::Tensor tokens = tokens_in.has_value() ? *tokens_in : at::Tensor();
     check_logprobs(logits, tokens, top, entropy);
     if (tokens.defined()) tokens = tokens.contiguous();
-    c10::optional<at::Tensor> none;
-    if (at::GradMode::is_enabled() && logits.requires_grad()) {
-        const variable_list out = TokenLogprobsFn::apply(logits, tokens, top, entropy);
-        size_t at = 0;
-        c10::optional<at::Tensor> lp = none, h = none, tl = none, tt = none;
-        if (tokens.defined()) lp = out[at++];
-        if (entropy) h = out[at++];
-        if (top > 0) {
-            tl = out[at++];
-            tt = out[at++];
-        }
-        return std::make_tuple(lp, h, tl, tt);
-    }
     const c10::DeviceGuard guard(logits.device());
-    const LogprobOutputs o = logprobs_forward(rows_of(logits), logits.sizes().slice(0, logits.dim() - 1), tokens, top, entropy, false);
+    const bool need = at::GradMode::is_enabled() && logits.requires_grad();
+    LogprobOutputs o;
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        o = logprobs_forward(rows_of(logits), logits.sizes().slice(0, logits.dim() - 1), tokens, top, entropy, need);
+    }
+    no_tangent("token_logprobs", logits);
+    if (need) {
+        const auto node = std::shared_ptr<TokenLogprobsBackward>(new TokenLogprobsBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(logits));
+        node->logits_ = SavedVariable(logits, false);
+        node->tokens_ = SavedVariable(tokens, false);
+        node->stats_ = SavedVariable(o.stats, false);
+        node->top_tokens_ = SavedVariable(o.top_tokens, false);
+        node->top = top;
+        node->has_logprobs = o.logprobs.defined();
+        node->has_entropy = o.entropy.defined();
+        for (at::Tensor *t : {&o.logprobs, &o.entropy, &o.top_logprobs})  // (the order of the gradients; the tokens have none)
+            if (t->defined()) torch::autograd::set_history(*t, node);
+    }
     const auto given = [](const at::Tensor &t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::optional<at::Tensor>(); };
     return std::make_tuple(given(o.logprobs), given(o.entropy), given(o.top_logprobs), given(o.top_tokens));
 }
@@ -205,35 +209,33 @@ at::Tensor embedding_forward(const at::Tensor &weight, const at::Tensor &tokens,
     return out;
 }
 
-struct TokenEmbeddingFn : public torch::autograd::Function<TokenEmbeddingFn> {
-    static at::Tensor forward(AutogradContext *ctx, at::Tensor weight, at::Tensor tokens, double scale, int64_t padding_idx) {
-        const c10::DeviceGuard guard(weight.device());
-        ctx->set_materialize_grads(false);
-        ctx->save_for_backward({tokens});
-        ctx->saved_data["scale"] = scale;
-        ctx->saved_data["padding_idx"] = padding_idx;
-        ctx->saved_data["V"] = weight.size(0);
-        return embedding_forward(weight, tokens, scale);
-    }
+struct TokenEmbeddingBackward : public Node {
+    SavedVariable tokens_;
+    double scale = 1.0;
+    int64_t padding_idx = -1, V = 0;
 
-    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    std::string name() const override { return "TokenEmbeddingBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        tokens_.reset_data();
+    }
+    variable_list apply(variable_list &&grads) override {
         const char *who = "token_embedding";
         no_second_derivative(who);
-        variable_list none(4);
-        if (!grads[0].defined()) return none;
-        const at::Tensor tokens = ctx->get_saved_variables()[0];
-        const int64_t V = ctx->saved_data["V"].toInt(), D = grads[0].size(-1), N = tokens.numel();
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (!task_should_compute_output(0) || !grads[0].defined()) return {at::Tensor()};
+        const at::Tensor tokens = tokens_.unpack();
+        const int64_t D = grads[0].size(-1), N = tokens.numel();
         const c10::DeviceGuard guard(tokens.device());
         // rows of D adjacent elements, the rows a fixed distance apart (0 for an expanded gradient)
-        at::Tensor g = grads[0].dim() == 2 && grads[0].stride(1) == 1 ? grads[0] : grads[0].contiguous().view({N, D});
+        const at::Tensor g = grads[0].dim() == 2 && grads[0].stride(1) == 1 ? grads[0] : grads[0].contiguous().view({N, D});
         const int64_t gstride = N > 1 ? g.stride(0) : D;
-        at::Tensor dw = at::empty({V, D}, g.options());
-        at::Tensor ws = at::empty({(int64_t)((pcfgnat_token_embedding_backward_workspace_bytes(N, V, D) + 7) / 8)}, g.options().dtype(at::kLong));
-        check_rc(pcfgnat_token_embedding_backward(g.data_ptr(), vocab_dtype(who, g), gstride, tokens.data_ptr<int64_t>(),
-                                                  (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding_idx"].toInt(),
-                                                  dw.data_ptr(), ws.data_ptr(), N, V, D, stream_of(g)));
-        none[0] = dw;
-        return none;
+        at::Tensor dw = at::empty({V, D}, g.options()), ws;
+        const int64_t nws = (int64_t)((pcfgnat_token_embedding_backward_workspace_bytes(vocab_dtype(who, g), N, V, D) + 7) / 8);
+        if (nws > 0) ws = at::empty({nws}, g.options().dtype(at::kLong));
+        check_rc(pcfgnat_token_embedding_backward(g.data_ptr(), vocab_dtype(who, g), gstride, tokens.data_ptr<int64_t>(), (float)scale, padding_idx,
+                                                  dw.data_ptr(), nws > 0 ? ws.data_ptr() : nullptr, N, V, D, stream_of(g)));
+        return {dw};
     }
 };
 
@@ -247,9 +249,23 @@ at::Tensor token_embedding(const at::Tensor &weight, const at::Tensor &tokens_in
     need_gpu(who, {&weight, &tokens_in});
     const at::Tensor tokens = tokens_in.contiguous();
     const int64_t pad = padding_idx.has_value() ? *padding_idx : -1;
-    if (at::GradMode::is_enabled() && weight.requires_grad()) return TokenEmbeddingFn::apply(weight, tokens, scale, pad);
     const c10::DeviceGuard guard(weight.device());
-    return embedding_forward(weight, tokens, scale);
+    at::Tensor out;
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        out = embedding_forward(weight, tokens, scale);
+    }
+    no_tangent(who, weight);
+    if (at::GradMode::is_enabled() && weight.requires_grad()) {
+        const auto node = std::shared_ptr<TokenEmbeddingBackward>(new TokenEmbeddingBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(weight));
+        node->tokens_ = SavedVariable(tokens, false);
+        node->scale = scale;
+        node->padding_idx = pad;
+        node->V = weight.size(0);
+        torch::autograd::set_history(out, node);
+    }
+    return out;
 }
 
 }  // namespace

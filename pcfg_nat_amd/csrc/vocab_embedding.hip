@@ -124,19 +124,23 @@ constexpr int SORT_U = 4;       // groups of 64 positions whose reads are on the
 // that the first has listed, or, where a wave has met more than its list holds (a common token), over all again.
 // The lanes that hold the same token are found by one ballot for each bit of the token; the last of them moves the token's
 // cursor on for all, so 64 positions cost the same whether they hold one token or 64.
-__global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t *__restrict__ tokens, int64_t padding_idx, int N, int64_t V,
-                                                                  int block_bits, int own_bits, int *__restrict__ count,
-                                                                  int *__restrict__ counts, int *__restrict__ starts,
-                                                                  int *__restrict__ order_pos, int *__restrict__ order_tok) {
-    extern __shared__ int s_at[];  // [SORT_NW][ids]: occurrences, then cursors
-    __shared__ unsigned s_list[SORT_NW][SORT_LIST];
-    __shared__ int s_below[SORT_NW], s_wave[SORT_NW];
+template <int NT>
+struct OrderShared {
+    unsigned list[NT / 64][SORT_LIST];
+    int below[NT / 64], wave[NT / 64];
+};
+// The work of one such workgroup of NT threads: its tokens are `block`, block + 2^block_bits, ..., `ids` <= NT of them.  s_at:
+// [NT / 64][ids] in LDS.  count(id, begin, n, before) is called by thread id, emit(place, position, id) for each of the own
+// tokens; begin and place count from this workgroup's first, `before` are the tokens of the workgroups before it.
+template <int NT, typename Count, typename Emit>
+__device__ __forceinline__ void order_own(const int64_t *__restrict__ tokens, int64_t padding_idx, int N, int64_t V, int block, int block_bits,
+                                          int own_bits, int ids, int *s_at, OrderShared<NT> &sh, Count count, Emit emit) {
+    constexpr int NW = NT / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int block = (int)blockIdx.x, block_mask = (1 << block_bits) - 1;
-    const int ids = (int)((V - block + block_mask) >> block_bits);
+    const int block_mask = (1 << block_bits) - 1;
     int *at_wave = s_at + wave * ids;
     for (int i = lane; i < ids; i += 64) at_wave[i] = 0;
-    const int groups = (int)(((int64_t)N + 63) / 64), each = (groups + SORT_NW - 1) / SORT_NW;
+    const int groups = (int)(((int64_t)N + 63) / 64), each = (groups + NW - 1) / NW;
     const int from = wave * each, to = from + each < groups ? from + each : groups;
     // goes over the wave's positions, a round of SORT_U groups at a time: f(token, the lanes that hold a real one, group).  The next
     // round's reads are ahead of what f stores, so that a wait for them (the hardware counts both in order) is none for the
@@ -178,7 +182,7 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
     // appends the own tokens of a group to the wave's list (a ring)
     const auto append = [&](uint64_t w, unsigned long long own, int g, int &listed) {
         if ((own >> lane) & 1)
-            s_list[wave][(listed + __popcll(own & ((1ull << lane) - 1))) & (SORT_LIST - 1)] =
+            sh.list[wave][(listed + __popcll(own & ((1ull << lane) - 1))) & (SORT_LIST - 1)] =
                 (unsigned)(w >> block_bits) << 22 | (unsigned)((g - from) * 64 + lane);
         listed += __popcll(own);
     };
@@ -192,46 +196,43 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
             if ((own >> lane) & 1) atomicAdd(&at_wave[w >> block_bits], 1);
             append(w, own, g, listed);
         });
-    if (lane == 0) s_below[wave] = below;
+    if (lane == 0) sh.below[wave] = below;
     __syncthreads();
     // exclusive sums over (token, wave)
     int mine = 0;
     if (tid < ids) {
 #pragma unroll
-        for (int w = 0; w < SORT_NW; w++) mine += s_at[w * ids + tid];
+        for (int w = 0; w < NW; w++) mine += s_at[w * ids + tid];
     }
     int upto = mine;
     for (int d = 1; d < 64; d <<= 1) {
         const int v = __shfl_up(upto, d);
         if (lane >= d) upto += v;
     }
-    if (lane == 63) s_wave[wave] = upto;
+    if (lane == 63) sh.wave[wave] = upto;
     __syncthreads();
     int base = upto - mine, all_before = 0, all_own = 0;
 #pragma unroll
-    for (int w = 0; w < SORT_NW; w++) {
-        all_before += s_below[w];
-        if (w < wave) base += s_wave[w];
-        all_own += s_wave[w];
+    for (int w = 0; w < NW; w++) {
+        all_before += sh.below[w];
+        if (w < wave) base += sh.wave[w];
+        all_own += sh.wave[w];
     }
-    base += all_before;
     if (tid < ids) {
         int at = base;
 #pragma unroll
-        for (int w = 0; w < SORT_NW; w++) {
-            const int c = s_at[w * ids + tid];
+        for (int w = 0; w < NW; w++) {
+            const int n = s_at[w * ids + tid];
             s_at[w * ids + tid] = at;
-            at += c;
+            at += n;
         }
-        counts[((int64_t)tid << block_bits) + block] = mine;
-        starts[((int64_t)tid << block_bits) + block] = base;
     }
-    if (block == block_mask && tid == 0) *count = all_before + all_own;
+    count(tid < ids ? tid : -1, base, mine, all_before, all_own);
     __syncthreads();
     // `n` listed tokens, from the first-th on, to their places
     const auto place = [&](int first, int n) {
         const bool own = lane < n;
-        const unsigned e = s_list[wave][(first + (own ? lane : 0)) & (SORT_LIST - 1)];
+        const unsigned e = sh.list[wave][(first + (own ? lane : 0)) & (SORT_LIST - 1)];
         const int id = (int)(e >> 22);
         unsigned long long same = __ballot(own);
         if (same & __ballot(id != __builtin_amdgcn_readfirstlane(id)))  // (one token alone is common: a run's)
@@ -245,8 +246,7 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
             const int at = __hip_atomic_load(&at_wave[id], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             const int rank = __popcll(same & ((1ull << lane) - 1)), all = __popcll(same);
             if (rank == all - 1) __hip_atomic_store(&at_wave[id], at + all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            order_pos[at + rank] = from * 64 + (int)(e & 0x3FFFFF);
-            order_tok[at + rank] = (id << block_bits) + block;
+            emit(at + rank, from * 64 + (int)(e & 0x3FFFFF), id);
         }
         __builtin_amdgcn_wave_barrier();
     };
@@ -266,6 +266,135 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
     }
     __builtin_amdgcn_wave_barrier();
     for (; placed < listed; placed += 64) place(placed, listed - placed < 64 ? listed - placed : 64);
+}
+
+__global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t *__restrict__ tokens, int64_t padding_idx, int N, int64_t V,
+                                                                  int block_bits, int own_bits, int *__restrict__ count,
+                                                                  int *__restrict__ counts, int *__restrict__ starts,
+                                                                  int *__restrict__ order_pos, int *__restrict__ order_tok) {
+    extern __shared__ int s_at[];  // [SORT_NW][ids]: occurrences, then cursors
+    __shared__ OrderShared<SORT_NT> sh;
+    const int block = (int)blockIdx.x, block_mask = (1 << block_bits) - 1;
+    const int ids = (int)((V - block + block_mask) >> block_bits);
+    int first = 0;
+    order_own<SORT_NT>(
+        tokens, padding_idx, N, V, block, block_bits, own_bits, ids, s_at, sh,
+        [&](int id, int begin, int n, int before, int own) {
+            first = before;
+            if (id >= 0) {
+                counts[((int64_t)id << block_bits) + block] = n;
+                starts[((int64_t)id << block_bits) + block] = before + begin;
+            }
+            if (block == block_mask && threadIdx.x == 0) *count = before + own;
+        },
+        [&](int place, int pos, int id) {
+            order_pos[first + place] = pos;
+            order_tok[first + place] = (id << block_bits) + block;
+        });
+}
+
+// Few positions: order and sums in one launch.  A workgroup owns up to 256 tokens of the vocabulary (as above) and 128 bytes
+// of columns, orders the positions of its tokens in LDS and sums: eight lanes a token, its rows in ascending position; a
+// token met more than HEAVY times by all the groups of eight, each every 32nd occurrence, and their sums in order.  Rows of
+// tokens that do not occur are zeroed.
+// Every workgroup looks at all positions, so this pays while these, times the tiles of columns, are few: 100 positions of
+// 40000 x 512 float16 take 11.9 us (in three launches 17.4 us), 8192 of 8000 x 128 bfloat16 13.0 us (17.0 us), but 5120 of
+// 40000 x 512 47 us (22.6 us).  The two launches saved are also 5 us of the host's time, which a small training step waits
+// for.  (Measured and dropped: this kernel's sums behind embedding_order_kernel, two launches: 40 us for those 5120.)
+constexpr int DIRECT_NT = 256, DIRECT_LANES = 8, DIRECT_GROUPS = DIRECT_NT / DIRECT_LANES;
+constexpr int DIRECT_TOKENS = 8192, HEAVY = 32;
+constexpr int64_t DIRECT_LOOKS = 16384, DIRECT_VOCAB = 1 << 18;
+inline int64_t direct_tiles(int es, int64_t D) { return (D * es + 16 * DIRECT_LANES - 1) / (16 * DIRECT_LANES); }
+inline bool direct_pays(int es, int64_t N, int64_t V, int64_t D) {
+    return D * es >= 16 && N <= DIRECT_TOKENS && V <= DIRECT_VOCAB && direct_tiles(es, D) <= DIRECT_LOOKS &&
+           N * direct_tiles(es, D) <= DIRECT_LOOKS;
+}
+template <typename T>
+__global__ __launch_bounds__(DIRECT_NT) void embedding_direct_kernel(const T *__restrict__ g, int64_t gstride, const int64_t *__restrict__ tokens,
+                                                                     float scale, int64_t padding_idx, T *__restrict__ dweight, int N, int64_t V,
+                                                                     int64_t D, int block_bits, int own_bits) {
+    constexpr int E = VocabElem<T>::N;
+    struct Sort {
+        OrderShared<DIRECT_NT> order;
+        int at[DIRECT_NT / 64 * DIRECT_NT];
+    };
+    __shared__ union {
+        Sort sort;
+        float sum[DIRECT_GROUPS][DIRECT_LANES * E];
+    } sh;
+    __shared__ int s_begin[DIRECT_NT], s_count[DIRECT_NT], s_heavy[DIRECT_TOKENS / HEAVY], s_heavies;
+    extern __shared__ unsigned short s_pos[];  // [N]
+    const int tid = threadIdx.x, lane = tid % DIRECT_LANES, group = tid / DIRECT_LANES;
+    const int block = (int)blockIdx.x, block_mask = (1 << block_bits) - 1;
+    const int ids = (int)((V - block + block_mask) >> block_bits);
+    if (tid == 0) s_heavies = 0;
+    __syncthreads();
+    order_own<DIRECT_NT>(
+        tokens, padding_idx, N, V, block, block_bits, own_bits, ids, sh.sort.at, sh.sort.order,
+        [&](int id, int begin, int n, int, int) {
+            if (id < 0) return;
+            s_begin[id] = begin;
+            s_count[id] = n;
+            if (n > HEAVY) s_heavy[atomicAdd(&s_heavies, 1)] = id;
+        },
+        [&](int place, int pos, int) { s_pos[place] = (unsigned short)pos; });
+    __syncthreads();
+    // (the last columns of D no multiple of a chunk: the row's last whole chunk, whose first columns a neighbour writes too)
+    const int64_t c0 = ((int64_t)blockIdx.y * DIRECT_LANES + lane) * E, c = c0 + E <= D ? c0 : D - E;
+    const bool live = c0 < D;
+    const auto row = [&](int j) { return *reinterpret_cast<const vec16_any *>(g + (int64_t)s_pos[j] * gstride + c); };
+    const auto add = [&](float (&acc)[E], const vec16 &v) {
+        float o[E];
+        VocabElem<T>::unpack(v, o);
+#pragma unroll
+        for (int k = 0; k < E; k++) acc[k] += o[k];
+    };
+    for (int i = group; i < ids; i += DIRECT_GROUPS) {
+        const int b = s_begin[i], n = s_count[i];
+        if (n > HEAVY) continue;
+        float acc[E];
+#pragma unroll
+        for (int k = 0; k < E; k++) acc[k] = 0.f;
+        constexpr int U = 4;
+        for (int j = 0; j < n; j += U) {
+            vec16 buf[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) buf[u] = row(b + (j + u < n ? j + u : n - 1));
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (j + u < n) add(acc, buf[u]);
+        }
+#pragma unroll
+        for (int k = 0; k < E; k++) acc[k] *= scale;
+        if (live) *reinterpret_cast<vec16_any *>(dweight + (((int64_t)i << block_bits) + block) * D + c) = VocabElem<T>::pack(acc);
+    }
+    const int heavies = s_heavies;
+    for (int h = 0; h < heavies; h++) {
+        const int i = s_heavy[h], b = s_begin[i], n = s_count[i];
+        float acc[E];
+#pragma unroll
+        for (int k = 0; k < E; k++) acc[k] = 0.f;
+        constexpr int U = 8;
+        for (int j = group; j < n; j += U * DIRECT_GROUPS) {
+            vec16 buf[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) buf[u] = row(b + (j + u * DIRECT_GROUPS < n ? j + u * DIRECT_GROUPS : n - 1));
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (j + u * DIRECT_GROUPS < n) add(acc, buf[u]);
+        }
+        __syncthreads();  // (the last heavy token's sums, or the order's lists, are done with)
+#pragma unroll
+        for (int k = 0; k < E; k++) sh.sum[group][lane * E + k] = acc[k];
+        __syncthreads();
+        if (tid < DIRECT_LANES * E) {
+            float all = 0.f;
+#pragma unroll
+            for (int w = 0; w < DIRECT_GROUPS; w++) all += sh.sum[w][tid];
+            const int64_t from = ((int64_t)blockIdx.y * DIRECT_LANES + tid / E) * E;
+            if (from < D) dweight[(((int64_t)i << block_bits) + block) * D + (from + E <= D ? from : D - E) + tid % E] = (T)(all * scale);
+        }
+    }
 }
 
 // A wave sums one piece of the order over a tile of 64 chunks of columns, 8 rows of g on their way at a time.  Runs that begin
@@ -398,11 +527,13 @@ __global__ __launch_bounds__(JOIN_NW * 64) void embedding_join_kernel(float scal
     }
 }
 
+constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;  // of 256 threads: a dimension of a grid ends at 2^32 threads
+
 template <typename T>
 int forward(const void *weight, int64_t wstride, const int64_t *tokens, float scale, void *out, int64_t N, int64_t V, int64_t D,
             hipStream_t s) {
     const int64_t each = 256 * LOOKUP_U * VocabElem<T>::N, blocks = (N * D + each - 1) / each;
-    PCFGNAT_REQUIRE(blocks <= 2147483647, "token_embedding: the output is too large for one call");
+    PCFGNAT_REQUIRE(blocks <= MAX_BLOCKS, "token_embedding: the output is too large for one call");
     if (D < VocabElem<T>::N)
         hipLaunchKernelGGL((embedding_fwd_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)weight, wstride, tokens, scale,
                            (T *)out, N, V, (unsigned)D);
@@ -415,21 +546,29 @@ int forward(const void *weight, int64_t wstride, const int64_t *tokens, float sc
 template <typename T>
 int backward(const void *g, int64_t gstride, const int64_t *tokens, float scale, int64_t padding_idx, void *dweight, void *workspace,
              int64_t N, int64_t V, int64_t D, hipStream_t s) {
+    const bool direct = direct_pays((int)sizeof(T), N, V, D);
+    // 256 workgroups own the vocabulary, fewer a smaller one, more where they would own too much each
+    int block_bits = 0, own_bits = 0;
+    while (block_bits < 8 && ((int64_t)2 << block_bits) <= V) block_bits++;
+    while (((V - 1) >> block_bits) + 1 > (direct ? DIRECT_NT : MAX_OWN)) block_bits++;
+    while (((int64_t)1 << own_bits) < ((V - 1) >> block_bits) + 1) own_bits++;
+    if (direct) {
+        hipLaunchKernelGGL(embedding_direct_kernel<T>, dim3(1u << block_bits, (unsigned)direct_tiles((int)sizeof(T), D)), dim3(DIRECT_NT),
+                           (size_t)(N + 1) * 2, s, (const T *)g, gstride, tokens, scale, padding_idx, (T *)dweight, (int)N, V, D, block_bits,
+                           own_bits);
+        PCFGNAT_HIP_CHECK(hipGetLastError());
+        return PCFGNAT_OK;
+    }
     const Plan p = plan_of(N, D);
     const int tiles = (int)((D + 64 * VocabElem<T>::N - 1) / (64 * VocabElem<T>::N));
     const int64_t sum_blocks = (p.pieces * tiles + (V + ZERO_ROWS - 1) / ZERO_ROWS + 3) / 4;
-    PCFGNAT_REQUIRE(sum_blocks <= 2147483647, "token_embedding_backward: the gradient is too large for one call");
+    PCFGNAT_REQUIRE(sum_blocks <= MAX_BLOCKS, "token_embedding_backward: the gradient is too large for one call");
     char *w = (char *)workspace;
     int *count = (int *)w, *order_pos = (int *)(w + 16), *order_tok = (int *)(w + 16 + order_bytes(p));
     int *counts = (int *)(w + 16 + 2 * order_bytes(p)), *starts = (int *)((char *)counts + align16((size_t)V * 4));
     float *cut = (float *)((char *)starts + align16((size_t)V * 4));
-    // 256 workgroups, fewer for a smaller vocabulary, more for one beyond 256 * MAX_OWN
-    int block_bits = 0, own_bits = 0;
-    while (block_bits < 8 && ((int64_t)2 << block_bits) <= V) block_bits++;
-    while (((V - 1) >> block_bits) + 1 > MAX_OWN) block_bits++;
-    while (((int64_t)1 << own_bits) < ((V - 1) >> block_bits) + 1) own_bits++;
     const size_t lds = (size_t)SORT_NW * (((V - 1) >> block_bits) + 1) * 4;
-    PCFGNAT_DYNAMIC_LDS(embedding_order_kernel, SORT_NW * MAX_OWN * 4);
+    if (lds > 48 * 1024) PCFGNAT_DYNAMIC_LDS(embedding_order_kernel, SORT_NW * MAX_OWN * 4);  // (with the static 16.5 KiB, what needs no leave)
     hipLaunchKernelGGL(embedding_order_kernel, dim3(1u << block_bits), dim3(SORT_NT), lds, s, tokens, padding_idx, (int)N, V, block_bits,
                        own_bits, count, counts, starts, order_pos, order_tok);
     PCFGNAT_HIP_CHECK(hipGetLastError());
@@ -471,8 +610,9 @@ extern "C" int pcfgnat_token_embedding(const void *weight, int dtype, int64_t we
     return forward<float>(weight, weight_stride, tokens, scale, out, N, V, D, s);
 }
 
-extern "C" size_t pcfgnat_token_embedding_backward_workspace_bytes(int64_t N, int64_t V, int64_t D) {
-    if (N < 0 || N > MAX_TOKENS || V < 1 || V > MAX_VOCAB || D < 1 || D > MAX_DIM) return 0;
+extern "C" size_t pcfgnat_token_embedding_backward_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
+    if (!vocab_dtype_ok(dtype) || N < 0 || N > MAX_TOKENS || V < 1 || V > MAX_VOCAB || D < 1 || D > MAX_DIM) return 0;
+    if (direct_pays(vocab_elem_bytes(dtype), N, V, D)) return 0;
     const Plan p = plan_of(N, D);
     return 16 + 2 * order_bytes(p) + 2 * align16((size_t)V * 4) + align16((size_t)p.pieces * 2 * D * 4);
 }
@@ -483,7 +623,9 @@ extern "C" int pcfgnat_token_embedding_backward(const void *grad_out, int dtype,
     PCFGNAT_REQUIRE(vocab_dtype_ok(dtype), "token_embedding_backward: the gradient must be float16, bfloat16 or float32");
     PCFGNAT_REQUIRE(N >= 0 && N <= MAX_TOKENS && V >= 1 && V <= MAX_VOCAB && D >= 1 && D <= MAX_DIM && grad_stride >= 0,
                     "token_embedding_backward: bad dimensions");
-    PCFGNAT_REQUIRE(grad_weight && workspace && (N == 0 || (grad_out && tokens)), "token_embedding_backward: null pointer");
+    PCFGNAT_REQUIRE(grad_weight && (N == 0 || (grad_out && tokens)) &&
+                        (workspace || pcfgnat_token_embedding_backward_workspace_bytes(dtype, N, V, D) == 0),
+                    "token_embedding_backward: null pointer");
     hipStream_t s = (hipStream_t)stream;
     if (dtype == PCFGNAT_F16) return backward<f16>(grad_out, grad_stride, tokens, scale, padding_idx, grad_weight, workspace, N, V, D, s);
     if (dtype == PCFGNAT_BF16) return backward<bf16>(grad_out, grad_stride, tokens, scale, padding_idx, grad_weight, workspace, N, V, D, s);

@@ -53,6 +53,13 @@ __device__ __forceinline__ unsigned long long wave_max_key(unsigned long long v)
     return v;
 }
 
+// The rows of a launch: x and y of the grid (a dimension of a grid ends at 2^32 threads), parts of a row z.
+constexpr int64_t GRID_X = 1 << 20;
+inline dim3 row_grid(int64_t rows, int64_t parts = 1) {
+    return dim3((unsigned)(rows < GRID_X ? rows : GRID_X), (unsigned)((rows + GRID_X - 1) / GRID_X), (unsigned)parts);
+}
+__device__ __forceinline__ unsigned row_of_grid() { return blockIdx.y * (unsigned)GRID_X + blockIdx.x; }
+
 // Row r of the logits.  (rows < 2^31: a 32-bit division, and none at all where one stride covers the rows)
 template <typename T>
 __device__ __forceinline__ const T *row_at(const T *logits, unsigned r, int64_t inner, int64_t so, int64_t si, bool one_stride) {
@@ -416,7 +423,8 @@ __device__ __forceinline__ void in_order(const unsigned long long *keys, int n, 
 template <typename T, int NT, int MAXC>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(MAXC >= 16 ? 4 : 1))) void logprobs_kernel(const T *__restrict__ logits, LogprobArgs a) {
     __shared__ Shared<NT> sh;
-    const unsigned r = blockIdx.x;
+    const unsigned r = row_of_grid();
+    if (r >= a.rows) return;
     const int tid = threadIdx.x;
     const int64_t tok = a.tokens ? a.tokens[r] : 0;
     if (tok < 0) {
@@ -444,8 +452,9 @@ template <typename T>
 __global__ __launch_bounds__(PART_NT) void logprobs_part_kernel(const T *__restrict__ logits, LogprobArgs a, int part_len,
                                                                 unsigned long long *__restrict__ work) {
     __shared__ Shared<PART_NT> sh;
-    const unsigned r = blockIdx.x;
-    const int part = blockIdx.y, parts = gridDim.y, tid = threadIdx.x;
+    const unsigned r = row_of_grid();
+    if (r >= a.rows) return;
+    const int part = blockIdx.z, parts = gridDim.z, tid = threadIdx.x;
     if (a.tokens && a.tokens[r] < 0) return;
     const int base = part * part_len;
     const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows) + base;
@@ -471,7 +480,8 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     __shared__ Shared<JOIN_NT> sh;
     __shared__ int s_lane[MAX_LANES];
     __shared__ int s_lanes;
-    const unsigned r = blockIdx.x;
+    const unsigned r = row_of_grid();
+    if (r >= a.rows) return;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int64_t tok = a.tokens ? a.tokens[r] : 0;
     if (tok < 0) {
@@ -608,7 +618,7 @@ inline Cut cut_of(int es, int64_t V) {
 
 template <typename T, int NT, int MAXC>
 void launch_rows(const T *x, const LogprobArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL((logprobs_kernel<T, NT, MAXC>), dim3((unsigned)a.rows), dim3(NT), 0, s, x, a);
+    hipLaunchKernelGGL((logprobs_kernel<T, NT, MAXC>), row_grid(a.rows), dim3(NT), 0, s, x, a);
 }
 template <typename T>
 int launch_forward(const void *logits, const LogprobArgs &a, void *work, hipStream_t s) {
@@ -617,9 +627,9 @@ int launch_forward(const void *logits, const LogprobArgs &a, void *work, hipStre
     const int chunks = (c.len + VocabElem<T>::N - 1) / VocabElem<T>::N;
     if (c.parts > 1) {
         unsigned long long *w = (unsigned long long *)work;
-        hipLaunchKernelGGL(logprobs_part_kernel<T>, dim3((unsigned)a.rows, (unsigned)c.parts), dim3(PART_NT), 0, s, x, a, c.len, w);
+        hipLaunchKernelGGL(logprobs_part_kernel<T>, row_grid(a.rows, c.parts), dim3(PART_NT), 0, s, x, a, c.len, w);
         PCFGNAT_HIP_CHECK(hipGetLastError());
-        hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3((unsigned)a.rows), dim3(JOIN_NT), 0, s, x, a, c.len, c.parts, w);
+        hipLaunchKernelGGL(logprobs_join_kernel<T>, row_grid(a.rows), dim3(JOIN_NT), 0, s, x, a, c.len, c.parts, w);
         PCFGNAT_HIP_CHECK(hipGetLastError());
         return PCFGNAT_OK;
     }
@@ -652,9 +662,10 @@ __global__ __launch_bounds__(NT) void logprobs_grad_kernel(const T *__restrict__
     __shared__ float s_g[MAX_TOP + 1];
     __shared__ int s_i[MAX_TOP + 1];
     __shared__ unsigned s_hit[NT * MAXC / 4];  // a byte for each chunk
-    const unsigned r = blockIdx.x;
+    const unsigned r = row_of_grid();
+    if (r >= a.rows) return;
     const int tid = threadIdx.x;
-    const int base = blockIdx.y * (NT * MAXC * N), n = a.V - base < NT * MAXC * N ? a.V - base : NT * MAXC * N;
+    const int base = blockIdx.z * (NT * MAXC * N), n = a.V - base < NT * MAXC * N ? a.V - base : NT * MAXC * N;
     T *dx = grad + (int64_t)r * a.V + base;
     const Span<T> sp(dx, n);
     vec16 *dv = reinterpret_cast<vec16 *>(dx + sp.head);
@@ -739,7 +750,7 @@ __global__ __launch_bounds__(NT) void logprobs_grad_kernel(const T *__restrict__
 template <typename T, int NT, int MAXC>
 void launch_grad_parts(const T *x, T *dx, const LogprobGradArgs &a, hipStream_t s) {
     const int part = NT * MAXC * VocabElem<T>::N;
-    hipLaunchKernelGGL((logprobs_grad_kernel<T, NT, MAXC>), dim3((unsigned)a.rows, (unsigned)((a.V + part - 1) / part)), dim3(NT), 0, s, x, dx, a);
+    hipLaunchKernelGGL((logprobs_grad_kernel<T, NT, MAXC>), row_grid(a.rows, (a.V + part - 1) / part), dim3(NT), 0, s, x, dx, a);
 }
 template <typename T>
 int launch_backward(const void *logits, void *grad, const LogprobGradArgs &a, hipStream_t s) {
@@ -751,8 +762,9 @@ int launch_backward(const void *logits, void *grad, const LogprobGradArgs &a, hi
 
 int check_sizes(const char *who, int dtype, int64_t outer, int64_t inner, int64_t so, int64_t si, int64_t V, int top) {
     PCFGNAT_REQUIRE(vocab_dtype_ok(dtype), "%s: logits must be float16, bfloat16 or float32", who);
-    PCFGNAT_REQUIRE(outer >= 0 && inner >= 0 && (outer == 0 || inner <= 2147483647 / outer) && V >= 1 && V <= MAX_LOGPROB_VOCAB && so >= 0 && si >= 0,
-                    "%s: bad dimensions", who);
+    PCFGNAT_REQUIRE(outer >= 0 && inner >= 0 && (outer == 0 || inner <= 2147483647 / outer) && V >= 1 && so >= 0 && si >= 0, "%s: bad dimensions",
+                    who);
+    PCFGNAT_REQUIRE(V <= MAX_LOGPROB_VOCAB, "%s: a vocabulary of at most %lld entries (got %lld)", who, (long long)MAX_LOGPROB_VOCAB, (long long)V);
     PCFGNAT_REQUIRE(top >= 0 && top <= MAX_TOP && top <= V, "%s: between 0 and %d alternatives, at most the vocabulary (got %d of %lld)", who,
                     MAX_TOP, top, (long long)V);
     return PCFGNAT_OK;

@@ -273,6 +273,9 @@ def test_logprobs_layouts(dtype):
     spaced = torch.stack([tokens, tokens], 1)[:, 0]
     assert spaced.stride(0) == 2
     run_logprobs(wide[:, :V], spaced, 0, True, True, gen)
+    empty = torch.empty((3, 0, 7), dtype=dtype, device=DEV, requires_grad=True)
+    ops.token_logprobs(empty, torch.empty((3, 0), dtype=torch.int64, device=DEV), top=2).logprobs.sum().backward()
+    assert empty.grad.shape == (3, 0, 7)
     none = ops.token_logprobs(torch.empty((0, 4, 7), dtype=dtype, device=DEV), torch.empty((0, 4), dtype=torch.int64, device=DEV), top=2)
     assert none.logprobs.shape == (0, 4) and none.top_tokens.shape == (0, 4, 2) and none.entropy is None
 
@@ -317,6 +320,11 @@ def test_logprobs_gradient_by_parts_and_by_differences():
     p = torch.softmax(x.double(), -1)
     p.scatter_add_(1, tokens[:, None], -torch.ones((rows, 1), dtype=torch.float64, device=DEV))
     assert (leaf.grad.double() + p).abs().max() <= 220 * U
+    got = ops.token_logprobs(leaf, tokens, top=top, entropy=True)  # twice through one graph: the same bits
+    loss = got.logprobs.sum() + got.entropy.sum() + got.top_logprobs.sum()
+    first, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    second, = torch.autograd.grad(loss, leaf)
+    assert torch.equal(first, second)
 
 
 @gpu
@@ -383,7 +391,7 @@ def run_embedding(V, D, tokens, dtype, scale, pad, gen, weight=None):
 @pytest.mark.parametrize("D", [1, 2, 3, 7, 8, 31, 64, 130, 512, 515, 1024, 2056])
 def test_embedding_sizes(D, dtype):
     gen = torch.Generator().manual_seed(D)
-    for V, N in ((1, 1), (5, 3), (67, 130), (300, 1000)):
+    for V, N in ((1, 1), (5, 3), (67, 130), (300, 1000), (300, 8193)):
         tokens = torch.randint(-1, V + 1, (N,), generator=gen).to(DEV)
         print("embedding V=%d N=%d D=%d %s" % (V, N, D, dtype), flush=True)
         run_embedding(V, D, tokens, dtype, 1.0, None, gen)
@@ -392,12 +400,13 @@ def test_embedding_sizes(D, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("N,D", [(4099, 72), (5000, 523), (9000, 72)])  # (in one launch, and in three)
 @pytest.mark.parametrize("kind", ["one", "two", "runs", "every", "reversed", "none", "pads", "ends"])
-def test_embedding_token_distributions(kind, dtype):
+def test_embedding_token_distributions(kind, N, D, dtype):
     """One token everywhere, two taking turns, runs, every row once, in reverse, no row at all, nearly all padding, the
     first and the last row."""
     gen = torch.Generator().manual_seed(2)
-    V, D, N = 4099, 72, 4099
+    V = N
     i = torch.arange(N)
     t = {"one": torch.full((N,), 17), "two": 5 + 4000 * (i % 2), "runs": i // 97, "every": i.clone(), "reversed": V - 1 - i,
          "none": torch.where(i % 2 == 0, torch.tensor(-1), torch.tensor(V)),
@@ -406,7 +415,7 @@ def test_embedding_token_distributions(kind, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("V,N", [(40000, 5120), (257, 70000), (250007, 3), (3, 33000), (70001, 20000)])
+@pytest.mark.parametrize("V,N", [(40000, 5120), (257, 70000), (250007, 3), (3, 33000), (70001, 20000), (300000, 50), (2, 8192), (65537, 8192)])
 def test_embedding_large(V, N):
     gen = torch.Generator().manual_seed(V)
     t = torch.where(torch.rand((N,), generator=gen) < 0.4, torch.tensor(min(3, V - 1)), torch.randint(0, V, (N,), generator=gen))
@@ -674,8 +683,31 @@ def test_offsets_beyond_32_bits():
 
 
 @gpu
+def test_more_rows_than_a_grid_dimension_has_waves():
+    """70 million rows of two entries: a wave each is more than 2^32 threads.  Whole results against the formulas."""
+    rows = 70000001
+    x = torch.randn((rows, 2), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).half()
+    tokens = torch.ones((rows,), dtype=torch.int64, device=DEV)
+    tokens[12345::1000] = -1
+    leaf = x.requires_grad_(True)
+    lp = ops.token_logprobs(leaf, tokens).logprobs
+    grad, = torch.autograd.grad(lp, leaf, torch.ones_like(lp))
+    live = tokens >= 0
+    d = (x.detach()[:, 0].float() - x.detach()[:, 1].float())
+    want = torch.where(live, -torch.nn.functional.softplus(d), torch.zeros_like(d))
+    # |log-probability| < 20 here: its own rounding and that of the comparison's formula, U (4 d + 220) each
+    assert (lp.detach() - want).abs().max() <= 2 * U * 300
+    p = torch.where(live, torch.sigmoid(d), torch.zeros_like(d))
+    for column, sign in ((0, -1.0), (1, 1.0)):
+        assert (grad[:, column].float() - sign * p).abs().max() <= half_step(torch.float16) + 2 * U * 600
+    del x, leaf, tokens, lp, grad, want, p, d, live
+    torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("N", [64, 8200])
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-def test_c_abi_with_results_at_any_element(dtype):
+def test_c_abi_with_results_at_any_element(dtype, N):
     """The entry points called directly, their results one element behind an aligned address; what lies around them stays."""
     lib = _lib.load()
     gen = torch.Generator().manual_seed(12)
@@ -695,14 +727,15 @@ def test_c_abi_with_results_at_any_element(dtype):
                                                    ups[0].data_ptr(), ups[1].data_ptr(), ups[2].data_ptr(), guard[1:].data_ptr(), V, stream), lib)
     assert guard[0] == 7 and guard[-1] == 7
     check_logprobs(x, tokens, 2, (lp, h, tl, tt), (guard[1:-1].view(rows, V), *ups))
-    vocab, D, N = 40, 29, 64
+    vocab, D = 40, 29
     weight = torch.randn((vocab, D), generator=gen).to(dtype).to(DEV)
     words = torch.randint(0, vocab // 2, (N,), generator=gen).to(DEV)
     out = torch.full((N * D + 2,), 7.0, dtype=dtype, device=DEV)
     _lib.check(lib.pcfgnat_token_embedding(weight.data_ptr(), code, D, words.data_ptr(), 2.0, out[1:].data_ptr(), N, vocab, D, stream), lib)
     dw = torch.full((vocab * D + 2,), 7.0, dtype=dtype, device=DEV)
     up = torch.randn((N, D), generator=gen).to(dtype).to(DEV)
-    need = lib.pcfgnat_token_embedding_backward_workspace_bytes(N, vocab, D)
+    need = lib.pcfgnat_token_embedding_backward_workspace_bytes(code, N, vocab, D)
+    assert (need == 0) == (N <= 8192)
     work = torch.full((need + 16,), 85, dtype=torch.uint8, device=DEV)
     _lib.check(lib.pcfgnat_token_embedding_backward(up.data_ptr(), code, D, words.data_ptr(), 2.0, -1, dw[1:].data_ptr(), work.data_ptr(), N, vocab,
                                                     D, stream), lib)
@@ -756,6 +789,7 @@ def test_c_abi_refusals_without_a_gpu():
     refused(logprobs(V=0), b"dimensions")
     refused(logprobs(outer=-1), b"dimensions")
     refused(logprobs(outer=1 << 20, inner=1 << 20), b"dimensions")
+    refused(logprobs(V=64 * 256 * 20 * 4 + 1), b"vocabulary of at most")
     refused(logprobs(top=9), b"alternatives")
     refused(logprobs(top=65, V=100), b"alternatives")
     refused(logprobs(logits=None), b"null")
@@ -782,6 +816,7 @@ def test_c_abi_refusals_without_a_gpu():
     refused(embed(V=0), b"dimensions")
     refused(embed(D=0), b"dimensions")
     refused(embed(N=-1), b"dimensions")
+    refused(embed(N=1 << 25, D=1 << 14, stride=1 << 14), b"too large")
     refused(embed(weight=None), b"null")
     assert embed(N=0) == _lib.OK
 
@@ -790,11 +825,14 @@ def test_c_abi_refusals_without_a_gpu():
 
     refused(embed_grad(dtype=_lib.F64), b"float16, bfloat16 or float32")
     refused(embed_grad(V=0), b"dimensions")
-    refused(embed_grad(N=1 << 33), b"dimensions")
+    refused(embed_grad(N=(16 << 22) + 1), b"dimensions")
+    refused(embed_grad(N=1 << 26, D=1 << 20), b"too large")
     refused(embed_grad(g=None), b"null")
     refused(embed_grad(out=None), b"null")
-    refused(embed_grad(ws=None), b"null")
-    assert lib.pcfgnat_token_embedding_backward_workspace_bytes(5120, 40000, 512) > 0
+    refused(embed_grad(N=9000, ws=None), b"null")
+    refused(embed_grad(N=8000, D=600, ws=None), b"null")
+    assert lib.pcfgnat_token_embedding_backward_workspace_bytes(_lib.F16, 51, 40000, 512) == 0  # in one launch
+    assert lib.pcfgnat_token_embedding_backward_workspace_bytes(_lib.F16, 51200, 40000, 512) > 0
 
 
 @gpu
