@@ -107,7 +107,9 @@ inline Plan plan_of(int64_t N, int64_t D) {
     return Plan{N, piece, (N + piece - 1) / piece};
 }
 // workspace: number of positions in the order (16 bytes), positions [N], tokens [N] in the order, occurrences and begin of
-// each token [V], [V], sums of cut runs [pieces][2][D] float32
+// each token [V], [V], sums of cut runs [pieces][2][D] float32; for many positions also tokens, positions and bounds of the
+// tiles spread over the owners
+inline bool spread_pays(int64_t N, int64_t V);
 inline size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 inline size_t order_bytes(const Plan &p) { return align16((size_t)p.N * 4); }
 
@@ -129,24 +131,23 @@ struct OrderShared {
     unsigned list[NT / 64][SORT_LIST];
     int below[NT / 64], wave[NT / 64];
 };
-// The work of one such workgroup of NT threads: its tokens are `block`, block + 2^block_bits, ..., `ids` <= NT of them.  s_at:
-// [NT / 64][ids] in LDS.  count(id, begin, n, before) is called by thread id, emit(place, position, id) for each of the own
-// tokens; begin and place count from this workgroup's first, `before` are the tokens of the workgroups before it.
-template <int NT, typename Count, typename Emit>
-__device__ __forceinline__ void order_own(const int64_t *__restrict__ tokens, int64_t padding_idx, int N, int64_t V, int block, int block_bits,
-                                          int own_bits, int ids, int *s_at, OrderShared<NT> &sh, Count count, Emit emit) {
-    constexpr int NW = NT / 64;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int block_mask = (1 << block_bits) - 1;
-    int *at_wave = s_at + wave * ids;
-    for (int i = lane; i < ids; i += 64) at_wave[i] = 0;
-    const int groups = (int)(((int64_t)N + 63) / 64), each = (groups + NW - 1) / NW;
-    const int from = wave * each, to = from + each < groups ? from + each : groups;
-    // goes over the wave's positions, a round of SORT_U groups at a time: f(token, the lanes that hold a real one, group).  The next
-    // round's reads are ahead of what f stores, so that a wait for them (the hardware counts both in order) is none for the
-    // stores.  Masks of lanes are scalar: a group is a handful of vector instructions where it holds none of the own tokens.
-    const uint64_t *words = reinterpret_cast<const uint64_t *>(tokens);
-    const auto look = [&](auto f) {
+// All positions, each wave its share: from * 64 up to to * 64.  The next round's reads are ahead of what f stores, so that a
+// wait for them (the hardware counts both in order) is none for the stores.  Masks of lanes are scalar: a group of 64 is a
+// handful of vector instructions where it holds none of the own tokens.
+template <int NT>
+struct LookAtAll {
+    const uint64_t *words;
+    int64_t padding_idx, V;
+    int N, from, to, lane;
+    __device__ __forceinline__ LookAtAll(const int64_t *tokens, int64_t padding, int n, int64_t v)
+        : words(reinterpret_cast<const uint64_t *>(tokens)), padding_idx(padding), V(v), N(n), lane((int)threadIdx.x & 63) {
+        const int groups = (int)(((int64_t)N + 63) / 64), each = (groups + NT / 64 - 1) / (NT / 64);
+        from = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * each;
+        to = from + each < groups ? from + each : groups;
+    }
+    template <typename F>
+    __device__ __forceinline__ void operator()(F f) const {
+        if (from >= to) return;
         uint64_t w[SORT_U], next[SORT_U];
         const auto load = [&](uint64_t (&to_w)[SORT_U], int g) {
             if (((int64_t)g + SORT_U) * 64 <= N) {
@@ -166,36 +167,56 @@ __device__ __forceinline__ void order_own(const int64_t *__restrict__ tokens, in
             load(next, g + SORT_U);
             if (g + SORT_U <= to && ((int64_t)g + SORT_U) * 64 <= N) {
 #pragma unroll
-                for (int u = 0; u < SORT_U; u++) f(w[u], __ballot(w[u] < (uint64_t)V) & __ballot(w[u] != (uint64_t)padding_idx), g + u);
+                for (int u = 0; u < SORT_U; u++)
+                    f(w[u], __ballot(w[u] < (uint64_t)V) & __ballot(w[u] != (uint64_t)padding_idx), (g + u - from) * 64 + lane);
             } else {
 #pragma unroll
                 for (int u = 0; u < SORT_U; u++) {
                     const int64_t left = g + u < to ? N - ((int64_t)g + u) * 64 : 0;
                     const unsigned long long there = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
-                    f(w[u], there & __ballot(w[u] < (uint64_t)V) & __ballot(w[u] != (uint64_t)padding_idx), g + u);
+                    f(w[u], there & __ballot(w[u] < (uint64_t)V) & __ballot(w[u] != (uint64_t)padding_idx), (g + u - from) * 64 + lane);
                 }
             }
 #pragma unroll
             for (int u = 0; u < SORT_U; u++) w[u] = next[u];
         }
-    };
+    }
+};
+
+// The work of one such workgroup of NT threads: its tokens are `block`, block + 2^block_bits, ..., `ids` <= NT of them.  s_at:
+// [NT / 64][ids] in LDS.  count(id, begin, n, before) is called by thread id, emit(place, position from the wave's first, id) for each of the own
+// tokens; begin and place count from this workgroup's first, `before` are the tokens of the workgroups before it.
+// `look(f)` calls f(token, the lanes that hold a real one, the lanes' positions counted from the wave's first) for all that
+// the wave has to look at, in ascending position.
+template <int NT, typename Look, typename Count, typename Emit>
+__device__ __forceinline__ void order_own(int block, int block_bits, int own_bits, int ids, int *s_at, OrderShared<NT> &sh, Look look, Count count,
+                                          Emit emit) {
+    constexpr int NW = NT / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int block_mask = (1 << block_bits) - 1;
+    int *at_wave = s_at + wave * ids;
+    for (int i = lane; i < ids; i += 64) at_wave[i] = 0;
     // appends the own tokens of a group to the wave's list (a ring)
-    const auto append = [&](uint64_t w, unsigned long long own, int g, int &listed) {
+    const auto append = [&](uint64_t w, unsigned long long own, int pos, int &listed) {
         if ((own >> lane) & 1)
             sh.list[wave][(listed + __popcll(own & ((1ull << lane) - 1))) & (SORT_LIST - 1)] =
-                (unsigned)(w >> block_bits) << 22 | (unsigned)((g - from) * 64 + lane);
+                (unsigned)(w >> block_bits) << 22 | (unsigned)pos;
         listed += __popcll(own);
     };
     int below = 0, listed = 0;
-    if (from < to)
-        look([&](uint64_t w, unsigned long long is, int g) {
-            const int owner = (int)w & block_mask;
-            below += __popcll(is & __ballot(owner < block));
-            const unsigned long long own = is & __ballot(owner == block);
-            if (own == 0) return;
-            if ((own >> lane) & 1) atomicAdd(&at_wave[w >> block_bits], 1);
-            append(w, own, g, listed);
-        });
+    look([&](uint64_t w, unsigned long long is, int pos) {
+        const int owner = (int)w & block_mask;
+        below += __popcll(is & __ballot(owner < block));
+        const unsigned long long own = is & __ballot(owner == block);
+        if (own == 0) return;
+        const int id = (int)(w >> block_bits), leader = __builtin_ctzll(own);
+        if (own & __ballot(id != __builtin_amdgcn_readlane(id, leader))) {
+            if ((own >> lane) & 1) atomicAdd(&at_wave[id], 1);
+        } else if (lane == leader) {  // one token alone is common: a run's; LDS takes additions to one place one after the other
+            atomicAdd(&at_wave[id], __popcll(own));
+        }
+        append(w, own, pos, listed);
+    });
     if (lane == 0) sh.below[wave] = below;
     __syncthreads();
     // exclusive sums over (token, wave)
@@ -235,7 +256,7 @@ __device__ __forceinline__ void order_own(const int64_t *__restrict__ tokens, in
         const unsigned e = sh.list[wave][(first + (own ? lane : 0)) & (SORT_LIST - 1)];
         const int id = (int)(e >> 22);
         unsigned long long same = __ballot(own);
-        if (same & __ballot(id != __builtin_amdgcn_readfirstlane(id)))  // (one token alone is common: a run's)
+        if (same & __ballot(id != __builtin_amdgcn_readfirstlane(id)))
             for (int bit = 0; bit < own_bits; bit++) {
                 const bool one = (id >> bit) & 1;
                 const unsigned long long set = __ballot(one);
@@ -246,17 +267,17 @@ __device__ __forceinline__ void order_own(const int64_t *__restrict__ tokens, in
             const int at = __hip_atomic_load(&at_wave[id], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             const int rank = __popcll(same & ((1ull << lane) - 1)), all = __popcll(same);
             if (rank == all - 1) __hip_atomic_store(&at_wave[id], at + all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            emit(at + rank, from * 64 + (int)(e & 0x3FFFFF), id);
+            emit(at + rank, (int)(e & 0x3FFFFF), id);
         }
         __builtin_amdgcn_wave_barrier();
     };
     int placed = 0;
     if (listed > SORT_LIST) {  // the list was overwritten: once more, placing 64 whenever there are
         listed = 0;
-        look([&](uint64_t w, unsigned long long is, int g) {
+        look([&](uint64_t w, unsigned long long is, int pos) {
             const unsigned long long own = is & __ballot(((int)w & block_mask) == block);
             if (own == 0) return;
-            append(w, own, g, listed);
+            append(w, own, pos, listed);
             if (listed - placed >= 64) {
                 __builtin_amdgcn_wave_barrier();
                 place(placed, 64);
@@ -276,9 +297,10 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
     __shared__ OrderShared<SORT_NT> sh;
     const int block = (int)blockIdx.x, block_mask = (1 << block_bits) - 1;
     const int ids = (int)((V - block + block_mask) >> block_bits);
+    const LookAtAll<SORT_NT> look(tokens, padding_idx, N, V);
     int first = 0;
     order_own<SORT_NT>(
-        tokens, padding_idx, N, V, block, block_bits, own_bits, ids, s_at, sh,
+        block, block_bits, own_bits, ids, s_at, sh, look,
         [&](int id, int begin, int n, int before, int own) {
             first = before;
             if (id >= 0) {
@@ -288,8 +310,148 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
             if (block == block_mask && threadIdx.x == 0) *count = before + own;
         },
         [&](int place, int pos, int id) {
-            order_pos[first + place] = pos;
+            order_pos[first + place] = look.from * 64 + pos;
             order_tok[first + place] = (id << block_bits) + block;
+        });
+}
+
+// Many positions: every workgroup looking at all of them is too much (131072 positions: 50 us and more), so they are first
+// spread over the owners.  A tile of SPREAD positions is brought into the order (owner, position) by a workgroup: places
+// among the tokens of one owner by ballots within the wave, by counts over waves and owners in LDS.  Leaves the tile's tokens
+// and positions in that order and where each owner's begin (one more for the end) ...
+constexpr int SPREAD_NT = 512, SPREAD_Q = 4, SPREAD = SPREAD_NT * SPREAD_Q, OWNERS = 256;
+constexpr int SPREAD_FROM = 16384;  // positions
+__global__ __launch_bounds__(SPREAD_NT) void embedding_spread_kernel(const int64_t *__restrict__ tokens, int64_t padding_idx, int N, int64_t V,
+                                                                     int *__restrict__ spread_tok, int *__restrict__ spread_pos,
+                                                                     int *__restrict__ bounds) {
+    constexpr int NW = SPREAD_NT / 64;
+    __shared__ int s_at[NW][OWNERS];
+    __shared__ int s_wave[OWNERS / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int i = lane; i < OWNERS; i += 64) s_at[wave][i] = 0;
+    const int64_t tile = blockIdx.x, at0 = tile * SPREAD + wave * (64 * SPREAD_Q) + lane;
+    uint64_t w[SPREAD_Q];
+#pragma unroll
+    for (int q = 0; q < SPREAD_Q; q++) w[q] = reinterpret_cast<const uint64_t *>(tokens)[at0 + q * 64 < N ? at0 + q * 64 : N - 1];
+    int place[SPREAD_Q];
+#pragma unroll
+    for (int q = 0; q < SPREAD_Q; q++) {
+        const bool real = at0 + q * 64 < N && w[q] < (uint64_t)V && w[q] != (uint64_t)padding_idx;
+        const int owner = (int)w[q] & (OWNERS - 1);
+        unsigned long long same = __ballot(real);
+#pragma unroll
+        for (int bit = 0; bit < 8; bit++) {
+            const bool one = (owner >> bit) & 1;
+            const unsigned long long set = __ballot(one);
+            same &= one ? set : ~set;
+        }
+        place[q] = -1;
+        if (real) {
+            // (this wave's counts alone; read by all lanes of the owner before the last of them writes)
+            const int at = __hip_atomic_load(&s_at[wave][owner], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            const int rank = __popcll(same & ((1ull << lane) - 1)), all = __popcll(same);
+            if (rank == all - 1) __hip_atomic_store(&s_at[wave][owner], at + all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            place[q] = at + rank;
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    int mine = 0, upto = 0;
+    if (tid < OWNERS) {
+#pragma unroll
+        for (int k = 0; k < NW; k++) {
+            const int c = s_at[k][tid];
+            s_at[k][tid] = mine;
+            mine += c;
+        }
+        upto = mine;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_up(upto, d);
+            if (lane >= d) upto += v;
+        }
+        if (lane == 63) s_wave[wave] = upto;
+    }
+    __syncthreads();
+    if (tid < OWNERS) {
+        int base = upto - mine;
+        for (int k = 0; k < wave; k++) base += s_wave[k];
+#pragma unroll
+        for (int k = 0; k < NW; k++) s_at[k][tid] += base;
+        int *out = bounds + tile * (OWNERS + 1);
+        out[tid] = base;
+        if (tid == OWNERS - 1) out[OWNERS] = base + mine;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < SPREAD_Q; q++)
+        if (place[q] >= 0) {
+            const int64_t to = tile * SPREAD + s_at[wave][(int)w[q] & (OWNERS - 1)] + place[q];
+            spread_tok[to] = (int)w[q];
+            spread_pos[to] = (int)(at0 + q * 64);
+        }
+}
+
+inline bool spread_pays(int64_t N, int64_t V) { return N > SPREAD_FROM && V >= OWNERS && V <= (int64_t)OWNERS * MAX_OWN; }
+inline size_t spread_bytes(int64_t N, int64_t V) {
+    if (!spread_pays(N, V)) return 0;
+    const size_t tiles = (size_t)((N + SPREAD - 1) / SPREAD);
+    return tiles * (2 * SPREAD + OWNERS + 1) * 4;
+}
+
+// ... and the owners order theirs, each wave a sixteenth of the tiles.
+__global__ __launch_bounds__(SORT_NT) void embedding_gather_kernel(const int *__restrict__ spread_tok, const int *__restrict__ spread_pos,
+                                                                   const int *__restrict__ bounds, int tiles, int64_t V, int own_bits,
+                                                                   int *__restrict__ count, int *__restrict__ counts, int *__restrict__ starts,
+                                                                   int *__restrict__ order_pos, int *__restrict__ order_tok) {
+    extern __shared__ int s_at[];  // [SORT_NW][ids]
+    __shared__ OrderShared<SORT_NT> sh;
+    __shared__ int s_before[SORT_NW];
+    const int block = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ids = (int)((V - block + OWNERS - 1) / OWNERS);
+    // tokens of the owners before this one: where its own begin, over all tiles
+    int before = 0;
+    for (int t = tid; t < tiles; t += SORT_NT) before += bounds[(int64_t)t * (OWNERS + 1) + block];
+    for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
+    if (lane == 0) s_before[wave] = before;
+    const int each = (tiles + SORT_NW - 1) / SORT_NW, t0 = wave * each, t1 = t0 + each < tiles ? t0 + each : tiles;
+    constexpr int U = 4;
+    const auto look = [&](auto f) {
+        for (int first = t0; first < t1; first += 64) {  // the bounds of 64 tiles at a time
+            const int64_t at = (int64_t)(first + lane < t1 ? first + lane : t1 - 1) * (OWNERS + 1) + block;
+            const int begins = bounds[at], ends = bounds[at + 1];
+            for (int t = first; t < first + 64 && t < t1; t++) {
+                const int begin = __builtin_amdgcn_readlane(begins, t - first), end = __builtin_amdgcn_readlane(ends, t - first);
+                for (int j = begin; j < end; j += 64 * U) {  // (a common token's owner: as many reads on their way together)
+                    int tok[U], pos[U];
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const int64_t e = (int64_t)t * SPREAD + (j + u * 64 + lane < end ? j + u * 64 + lane : end - 1);
+                        tok[u] = spread_tok[e];
+                        pos[u] = spread_pos[e];
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const int left = end - j - u * 64;
+                        if (left > 0) f((uint64_t)(unsigned)tok[u], left >= 64 ? ~0ull : (1ull << left) - 1, pos[u] - t0 * SPREAD);
+                    }
+                }
+            }
+        }
+    };
+    int first = 0;
+    order_own<SORT_NT>(
+        block, 8, own_bits, ids, s_at, sh, look,
+        [&](int id, int begin, int n, int, int own) {
+            for (int w = 0; w < SORT_NW; w++) first += s_before[w];
+            if (id >= 0) {
+                counts[(int64_t)id * OWNERS + block] = n;
+                starts[(int64_t)id * OWNERS + block] = first + begin;
+            }
+            if (block == OWNERS - 1 && tid == 0) *count = first + own;
+        },
+        [&](int place, int pos, int id) {
+            order_pos[first + place] = t0 * SPREAD + pos;
+            order_tok[first + place] = id * OWNERS + block;
         });
 }
 
@@ -329,15 +491,16 @@ __global__ __launch_bounds__(DIRECT_NT) void embedding_direct_kernel(const T *__
     const int ids = (int)((V - block + block_mask) >> block_bits);
     if (tid == 0) s_heavies = 0;
     __syncthreads();
+    const LookAtAll<DIRECT_NT> look(tokens, padding_idx, N, V);
     order_own<DIRECT_NT>(
-        tokens, padding_idx, N, V, block, block_bits, own_bits, ids, sh.sort.at, sh.sort.order,
+        block, block_bits, own_bits, ids, sh.sort.at, sh.sort.order, look,
         [&](int id, int begin, int n, int, int) {
             if (id < 0) return;
             s_begin[id] = begin;
             s_count[id] = n;
             if (n > HEAVY) s_heavy[atomicAdd(&s_heavies, 1)] = id;
         },
-        [&](int place, int pos, int) { s_pos[place] = (unsigned short)pos; });
+        [&](int place, int pos, int) { s_pos[place] = (unsigned short)(look.from * 64 + pos); });
     __syncthreads();
     // (the last columns of D no multiple of a chunk: the row's last whole chunk, whose first columns a neighbour writes too)
     const int64_t c0 = ((int64_t)blockIdx.y * DIRECT_LANES + lane) * E, c = c0 + E <= D ? c0 : D - E;
@@ -568,9 +731,23 @@ int backward(const void *g, int64_t gstride, const int64_t *tokens, float scale,
     int *counts = (int *)(w + 16 + 2 * order_bytes(p)), *starts = (int *)((char *)counts + align16((size_t)V * 4));
     float *cut = (float *)((char *)starts + align16((size_t)V * 4));
     const size_t lds = (size_t)SORT_NW * (((V - 1) >> block_bits) + 1) * 4;
-    if (lds > 48 * 1024) PCFGNAT_DYNAMIC_LDS(embedding_order_kernel, SORT_NW * MAX_OWN * 4);  // (with the static 16.5 KiB, what needs no leave)
-    hipLaunchKernelGGL(embedding_order_kernel, dim3(1u << block_bits), dim3(SORT_NT), lds, s, tokens, padding_idx, (int)N, V, block_bits,
-                       own_bits, count, counts, starts, order_pos, order_tok);
+    if (lds > 47 * 1024) {  // (with the static 16.6 KiB, what needs no leave)
+        PCFGNAT_DYNAMIC_LDS(embedding_order_kernel, SORT_NW * MAX_OWN * 4);
+        PCFGNAT_DYNAMIC_LDS(embedding_gather_kernel, SORT_NW * MAX_OWN * 4);
+    }
+    if (spread_pays(N, V)) {
+        const int64_t tiles = (N + SPREAD - 1) / SPREAD;
+        int *spread_tok = (int *)((char *)cut + align16((size_t)p.pieces * 2 * D * 4)), *spread_pos = spread_tok + tiles * SPREAD;
+        int *bounds = spread_pos + tiles * SPREAD;
+        hipLaunchKernelGGL(embedding_spread_kernel, dim3((unsigned)tiles), dim3(SPREAD_NT), 0, s, tokens, padding_idx, (int)N, V, spread_tok,
+                           spread_pos, bounds);
+        PCFGNAT_HIP_CHECK(hipGetLastError());
+        hipLaunchKernelGGL(embedding_gather_kernel, dim3(OWNERS), dim3(SORT_NT), lds, s, spread_tok, spread_pos, bounds, (int)tiles, V, own_bits,
+                           count, counts, starts, order_pos, order_tok);
+    } else {
+        hipLaunchKernelGGL(embedding_order_kernel, dim3(1u << block_bits), dim3(SORT_NT), lds, s, tokens, padding_idx, (int)N, V, block_bits,
+                           own_bits, count, counts, starts, order_pos, order_tok);
+    }
     PCFGNAT_HIP_CHECK(hipGetLastError());
     if (D < VocabElem<T>::N)
         hipLaunchKernelGGL((embedding_sum_kernel<T, true>), dim3((unsigned)sum_blocks), dim3(256), 0, s, (const T *)g, gstride, scale,
@@ -614,7 +791,7 @@ extern "C" size_t pcfgnat_token_embedding_backward_workspace_bytes(int dtype, in
     if (!vocab_dtype_ok(dtype) || N < 0 || N > MAX_TOKENS || V < 1 || V > MAX_VOCAB || D < 1 || D > MAX_DIM) return 0;
     if (direct_pays(vocab_elem_bytes(dtype), N, V, D)) return 0;
     const Plan p = plan_of(N, D);
-    return 16 + 2 * order_bytes(p) + 2 * align16((size_t)V * 4) + align16((size_t)p.pieces * 2 * D * 4);
+    return 16 + 2 * order_bytes(p) + 2 * align16((size_t)V * 4) + align16((size_t)p.pieces * 2 * D * 4) + align16(spread_bytes(N, V));
 }
 
 extern "C" int pcfgnat_token_embedding_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, float scale,

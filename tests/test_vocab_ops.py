@@ -400,7 +400,7 @@ def test_embedding_sizes(D, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("N,D", [(4099, 72), (5000, 523), (9000, 72)])  # (in one launch, and in three)
+@pytest.mark.parametrize("N,D", [(4099, 72), (5000, 523), (9000, 72), (17001, 8)])  # (in one, three, three and four launches)
 @pytest.mark.parametrize("kind", ["one", "two", "runs", "every", "reversed", "none", "pads", "ends"])
 def test_embedding_token_distributions(kind, N, D, dtype):
     """One token everywhere, two taking turns, runs, every row once, in reverse, no row at all, nearly all padding, the
@@ -415,7 +415,7 @@ def test_embedding_token_distributions(kind, N, D, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("V,N", [(40000, 5120), (257, 70000), (250007, 3), (3, 33000), (70001, 20000), (300000, 50), (2, 8192), (65537, 8192)])
+@pytest.mark.parametrize("V,N", [(40000, 5120), (257, 70000), (250007, 3), (3, 33000), (70001, 20000), (300000, 50), (2, 8192), (65537, 8192), (300000, 20000), (256, 16385), (262144, 18433)])
 def test_embedding_large(V, N):
     gen = torch.Generator().manual_seed(V)
     t = torch.where(torch.rand((N,), generator=gen) < 0.4, torch.tensor(min(3, V - 1)), torch.randint(0, V, (N,), generator=gen))
