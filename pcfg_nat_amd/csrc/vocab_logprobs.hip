@@ -45,14 +45,6 @@ __device__ __forceinline__ float value_of_order(unsigned o) { return __uint_as_f
 __device__ __forceinline__ float value_of(unsigned long long key) { return value_of_order((unsigned)(key >> 32)); }
 __device__ __forceinline__ int index_of(unsigned long long key) { return (int)(0xFFFFFFFEu - (unsigned)key); }
 
-__device__ __forceinline__ unsigned long long wave_max_key(unsigned long long v) {
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned long long w = __shfl_xor(v, o);
-        v = w > v ? w : v;
-    }
-    return v;
-}
-
 // The rows of a launch: x and y of the grid (a dimension of a grid ends at 2^32 threads), parts of a row z.
 constexpr int64_t GRID_X = 1 << 20;
 inline dim3 row_grid(int64_t rows, int64_t parts = 1) {
@@ -108,49 +100,92 @@ __device__ __forceinline__ int block_count(int v, Shared<NT> &sh, int tid) {
     return t;
 }
 
-// Calls f(value, index) for the elements of a span, reading them from memory.
-template <typename T, int NT, typename F>
-__device__ __forceinline__ void for_each(const T *x, const Span<T> &sp, int tid, F f) {
-    constexpr int N = VocabElem<T>::N;
-    const int e = sp.edge(tid);
-    if (e >= 0) f((float)x[e], e);
-    const vec16 *xv = reinterpret_cast<const vec16 *>(x + sp.head);
-    for (int c = tid; c < sp.nvec; c += NT) {
-        float o[N];
-        VocabElem<T>::unpack(xv[c], o);
-        for (int i = 0; i < N; i++) f(o[i], sp.head + c * N + i);
+// Appends the keys of those of N values (indexes first, first + 1, ...) that `want` names to the list, as far as it goes; their
+// number is counted on.
+template <int NT, int N, typename Want>
+__device__ __forceinline__ void append_keys(Shared<NT> &sh, const float (&o)[N], int first, Want want) {
+    unsigned which = 0;
+#pragma unroll
+    for (int k = 0; k < N; k++) which |= want(o[k]) ? 1u << k : 0u;
+    if (which == 0) return;
+    int at = atomicAdd(&sh.n, __popc(which));
+#pragma unroll
+    for (int k = 0; k < N; k++)
+        if (which & (1u << k)) {
+            if (at < Shared<NT>::MAX_KEYS) sh.key[at] = key_of(o[k], first + k);
+            at++;
+        }
+}
+
+// The q-th largest of a wave's values, which hold no NaN; equal ones are counted one by one.  (A wave that has fewer than q
+// values above -inf: -inf.)
+__device__ __forceinline__ float wave_nth_largest(float v, float largest, int q) {
+    for (;;) {
+        const int equal = __popcll(__ballot(v == largest));
+        q -= equal > 0 ? equal : 1;
+        if (q <= 0) return largest;
+        v = v == largest ? NEG_INF_F : v;
+        largest = wave_max_raw(v);
     }
 }
 
-// The `want` largest of a span whatever it holds (NaN, a constant, a mask that leaves fewer than `want`): the threshold t,
-// the want-th largest in the order of `order_of`, bit by bit - `guess` first, which is it where most of the span is one
-// value -, then everything above t (fewer than `want`), then the lowest indexes of those equal to t.  Reads the span again
-// for each step; rows of ordinary logits never come here.  Leaves `want` keys in sh.key.
-template <typename T, int NT>
-__device__ __forceinline__ void select_any(const T *x, const Span<T> &sp, int want, unsigned guess, Shared<NT> &sh, int tid) {
-    constexpr int N = VocabElem<T>::N;
-    const auto count_from = [&](unsigned t) {
-        int k = 0;
-        for_each<T, NT>(x, sp, tid, [&](float v, int) { k += order_of(v) >= t ? 1 : 0; });
-        return block_count<NT>(k, sh, tid);
-    };
-    unsigned t = 0;
-    if (count_from(guess) >= want && (guess == 0xFFFFFFFFu || count_from(guess + 1) < want)) {
-        t = guess;
-    } else {
-        for (unsigned bit = 0x80000000u; bit != 0; bit >>= 1)
-            if (count_from(t | bit) >= want) t |= bit;
+// Calls f(the values of a chunk, or the one of the scalar besides; their first index) for the elements of a span, reading them
+// from memory, two chunks a thread on their way at once.
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void for_each(const T *x, const Span<T> &sp, int tid, F f) {
+    constexpr int N = VocabElem<T>::N, U = 2;
+    const int e = sp.edge(tid);
+    if (e >= 0) {
+        const float o[1] = {(float)x[e]};
+        f(o, e);
     }
-    __syncthreads();
-    if (tid == 0) sh.n = 0;
-    __syncthreads();
-    for_each<T, NT>(x, sp, tid, [&](float v, int i) {
-        if (order_of(v) > t) sh.key[atomicAdd(&sh.n, 1)] = key_of(v, i);
-    });
-    __syncthreads();
-    int n = sh.n;
-    // ties in ascending index: the head, rounds of one chunk a thread, the tail
     const vec16 *xv = reinterpret_cast<const vec16 *>(x + sp.head);
+    for (int c = tid; c < sp.nvec; c += U * NT) {
+        vec16 v[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) v[u] = xv[c + u * NT < sp.nvec ? c + u * NT : c];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (c + u * NT < sp.nvec) {
+                float o[N];
+                VocabElem<T>::unpack(v[u], o);
+                f(o, sp.head + (c + u * NT) * N);
+            }
+    }
+}
+
+// The `want` largest of a span whatever it holds (NaN, a constant, a mask that leaves fewer than `want`), where at least `want`
+// elements lie at or above `guess` in the order of `order_of`.  Everything above the guess is listed: where that is at least
+// `want` and fits (a NaN among ordinary logits) nothing else is done; where it is fewer (most of the span is one value, a
+// mask's) the lowest indexes of those equal to the guess follow.  Otherwise the want-th largest is found bit by bit first.
+// Reads the span again for each step.  Returns how many keys it leaves in sh.key, `want` or more.
+template <typename T, int NT>
+__device__ __forceinline__ int select_any(const T *x, const Span<T> &sp, int want, unsigned guess, Shared<NT> &sh, int tid) {
+    constexpr int N = VocabElem<T>::N;
+    const vec16 *xv = reinterpret_cast<const vec16 *>(x + sp.head);
+    const auto list_above = [&](unsigned t) {
+        __syncthreads();
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        for_each<T, NT>(x, sp, tid, [&](const auto &o, int first) { append_keys<NT>(sh, o, first, [&](float v) { return order_of(v) > t; }); });
+        __syncthreads();
+        return sh.n;
+    };
+    unsigned t = guess;
+    int n = list_above(t);  // (the same for every thread)
+    if (n > Shared<NT>::MAX_KEYS) {
+        t = 0;
+        for (unsigned bit = 0x80000000u; bit != 0; bit >>= 1) {
+            int k = 0;
+            for_each<T, NT>(x, sp, tid, [&](const auto &o, int) {
+                for (const float v : o) k += order_of(v) >= (t | bit) ? 1 : 0;
+            });
+            if (block_count<NT>(k, sh, tid) >= want) t |= bit;
+        }
+        n = list_above(t);
+    }
+    const int above = n;
+    // ties in ascending index: the head, rounds of one chunk a thread, the tail
     const int rounds = (sp.nvec + NT - 1) / NT;
     for (int round = -1; round <= rounds && n < want; round++) {
         float o[N];
@@ -189,6 +224,7 @@ __device__ __forceinline__ void select_any(const T *x, const Span<T> &sp, int wa
         n += all;
         __syncthreads();
     }
+    return above < want ? want : above;
 }
 
 // What one workgroup finds in its part of a row, in base 2: z = sum of 2^t, s = sum of 2^t t, where t = (x - m) log2 e + shift.
@@ -202,11 +238,12 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // read once, all loads on their way together.
 //
 // Sums: one fused multiply-add (which also widens a float16), one exponential, one addition and one multiply-add an
-// element.  Where an entry is -inf its t is too and s becomes NaN although z does not; such rows, and those whose maximum
-// is so large that m log2 e could leave float32, take the careful form, whose t is clamped.
+// element.  Where an entry is -inf its t is too and s becomes NaN; a wave that finds one forms its s again from the
+// registers, with t clamped.  Rows whose largest entry is so large that m log2 e could leave float32 take the careful form,
+// which reads them again.
 //
-// Alternatives: from every wave the q-th largest of its lanes' maxima (q = top / waves, rounded up), the lowest of them
-// over the waves: at least `top` elements lie at or above it, and of ordinary logits hardly more (some 30 for 20 of
+// Alternatives: from every wave the q-th largest of its lanes' maxima (q = top / waves, rounded up), equal ones counted one by
+// one, the lowest of them over the waves: at least `top` elements lie at or above it, and of ordinary logits hardly more (some 30 for 20 of
 // 40000).  The chunks that hold one are known from the first pass's maxima; they alone are read again and their candidates
 // listed, to be put in order by counting.  What overflows the list (a constant, a mask) or holds a NaN goes to select_any.
 // Leaves in sh.key[0..kept) the keys of the candidates, all of the `top` largest among them.
@@ -265,11 +302,7 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int top, bool keep,
         }
         tau = t > LOWEST_ORDER ? value_of_order(t) : NEG_INF_F;
     } else if (top > 0) {
-        float rest = mine;
-        for (int q = (top + NW - 1) / NW; q > 1; q--) {
-            rest = rest == tau ? NEG_INF_F : rest;
-            tau = wave_max_raw(rest);
-        }
+        tau = wave_nth_largest(mine, m, (top + NW - 1) / NW);
     }
     if (lane == 0) {
         sh.max[wave] = m;
@@ -293,7 +326,7 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int top, bool keep,
     }
     const float mm = m == NEG_INF_F ? 0.f : m;
     float z = 0.f, s = 0.f, shift = 0.f;
-    bool careful = !(fabsf(mm) < 1e30f);
+    const bool careful = !(fabsf(mm) < 1e30f);
     if (!careful) {
         const float nb = -(mm * LOG2E);
         shift = __builtin_fmaf(mm, LOG2E, nb);
@@ -316,67 +349,81 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int top, bool keep,
                 }
             }
         }
+        if (__ballot(s != s) != 0) {
+            s = 0.f;
+            const auto add = [&](float v) {
+                const float t = __builtin_fmaf(v, LOG2E, nb);
+                s = __builtin_fmaf(__builtin_amdgcn_exp2f(t), fmaxf(t, -1e30f), s);
+            };
+            if (ei >= 0) add(edge);
+#pragma unroll
+            for (int i = 0; i < MAXC; i++) {
+                opaque(buf[i]);
+                if (tid + i * NT < sp.nvec) {
+                    float o[N];
+                    VocabElem<T>::unpack(buf[i], o);
+#pragma unroll
+                    for (int k = 0; k < N; k++) add(o[k]);
+                }
+            }
+        }
     }
     if (top > 0) {
         const auto take = [&](float v, int i) {
             if (v >= tau) {
                 const int at = atomicAdd(&sh.n, 1);
                 if (at < Shared<NT>::MAX_KEYS) sh.key[at] = key_of(v, i);
+                else hold = 0;  // (too many: not worth the rest)
             }
         };
         if (ei >= 0) take(edge, ei);
+        float o[N];
         if (MAXC <= FEW) {
 #pragma unroll
             for (int i = 0; i < MAXC; i++)
                 if (hold & (1u << i)) {
-                    const typename VocabElem<T>::vecT t = __builtin_bit_cast(typename VocabElem<T>::vecT, buf[i]);
+                    VocabElem<T>::unpack(buf[i], o);
 #pragma unroll
-                    for (int k = 0; k < N; k++) take((float)t[k], sp.head + (tid + i * NT) * N + k);
+                    for (int k = 0; k < N; k++) take(o[k], sp.head + (tid + i * NT) * N + k);
                 }
         } else {
             while (hold) {
                 const int c = tid + __builtin_ctz(hold) * NT;
-                const typename VocabElem<T>::vecT t = __builtin_bit_cast(typename VocabElem<T>::vecT, held);
+                VocabElem<T>::unpack(held, o);
                 hold &= hold - 1;
                 if (hold) held = xv[tid + __builtin_ctz(hold) * NT];
 #pragma unroll
-                for (int k = 0; k < N; k++) take((float)t[k], sp.head + c * N + k);
+                for (int k = 0; k < N; k++) take(o[k], sp.head + c * N + k);
             }
         }
     }
-    for (bool again = careful;;) {  // (everything here is the same for every thread)
-        if (again) {
-            z = s = shift = 0.f;
-            for_each<T, NT>(x, sp, tid, [&](float v, int) {
+    if (careful)  // (the same for every thread)
+        for_each<T, NT>(x, sp, tid, [&](const auto &o, int) {
+            for (const float v : o) {
                 const float d = v - mm, e = __builtin_amdgcn_exp2f(d * LOG2E);
                 z += e;
                 s = __builtin_fmaf(e, fmaxf(d, -1e30f) * LOG2E, s);
-            });
-        }
-        z = wave_sum(z);
-        s = wave_sum(s);
-        if (lane == 0) {
-            sh.z[wave] = z;
-            sh.s[wave] = s;
-        }
-        __syncthreads();
-        z = sh.z[0];
-        s = sh.s[0];
+            }
+        });
+    z = wave_sum(z);
+    s = wave_sum(s);
+    if (lane == 0) {
+        sh.z[wave] = z;
+        sh.s[wave] = s;
+    }
+    __syncthreads();
+    z = sh.z[0];
+    s = sh.s[0];
 #pragma unroll
-        for (int w = 1; w < NW; w++) {
-            z += sh.z[w];
-            s += sh.s[w];
-        }
-        if (again || !(s != s && z == z)) break;
-        again = true;
-        __syncthreads();
+    for (int w = 1; w < NW; w++) {
+        z += sh.z[w];
+        s += sh.s[w];
     }
     if (top > 0) {
         const int want = top < n ? top : n;
         kept = sh.n;
         if (kept > Shared<NT>::MAX_KEYS || kept < want || z != z) {  // (the same for every thread)
-            kept = want;
-            select_any<T, NT>(x, sp, kept, order_of(tau), sh, tid);
+            kept = select_any<T, NT>(x, sp, want, order_of(tau), sh, tid);
         }
     }
     return Part{m, z, s, shift};
@@ -471,7 +518,7 @@ __global__ __launch_bounds__(PART_NT) void logprobs_part_kernel(const T *__restr
 // ... and a workgroup per row joins the sums, rescaled to the row's maximum, and finds the alternatives: a threshold from the
 // lanes' maxima as scan_part takes it from its own, the lanes at or above it (hardly more than `top` of some thousand),
 // whose elements alone are read again, their candidates in order.  (Ordered lists from every part instead: 64 alternatives
-// of 64 rows of 250007 float32 in 38 us instead of NEW us.)
+// of 64 rows of 250007 float32 in 38 us instead of 25 us.)
 constexpr int JOIN_NT = 1024;
 template <typename T>
 __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restrict__ logits, LogprobArgs a, int part_len, int parts,
@@ -530,11 +577,7 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
 #pragma unroll
     for (int u = 0; u < U; u++) mine = max2_raw(mine, v[u]);
     for (int l0 = tid + U * JOIN_NT; l0 < all; l0 += JOIN_NT) mine = max2_raw(mine, lane_max(l0));
-    float tau = wave_max_raw(mine), rest = mine;
-    for (int q = (a.top + NW - 1) / NW; q > 1; q--) {
-        rest = rest == tau ? NEG_INF_F : rest;
-        tau = wave_max_raw(rest);
-    }
+    float tau = wave_nth_largest(mine, wave_max_raw(mine), (a.top + NW - 1) / NW);
     if (lane == 0) sh.tau[wave] = tau;
     if (tid == 0) sh.n = s_lanes = 0;
     __syncthreads();
@@ -554,7 +597,7 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     const int lanes = s_lanes;
     bool fits = lanes <= MAX_LANES && z == z;
     if (fits) {
-        const auto candidate = [&](float v, int i) {
+        const auto take = [&](float v, int i) {
             if (v >= tau) {
                 const int at = atomicAdd(&sh.n, 1);
                 if (at < Shared<JOIN_NT>::MAX_KEYS) sh.key[at] = key_of(v, i);
@@ -575,7 +618,7 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
                 const Span<T> sp(x + base, n);
                 if (k == PART_MAXC) {
                     const int e = sp.edge(t);
-                    if (e >= 0) candidate((float)x[base + e], base + e);
+                    if (e >= 0) take((float)x[base + e], base + e);
                 } else if (t + k * PART_NT < sp.nvec) {
                     at[u] = base + sp.head + (t + k * PART_NT) * N;
                     v[u] = *reinterpret_cast<const vec16 *>(x + at[u]);
@@ -584,17 +627,17 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
 #pragma unroll
             for (int u = 0; u < 4; u++)
                 if (at[u] >= 0) {
-                    const typename VocabElem<T>::vecT w = __builtin_bit_cast(typename VocabElem<T>::vecT, v[u]);
+                    float o[N];
+                    VocabElem<T>::unpack(v[u], o);
 #pragma unroll
-                    for (int k = 0; k < N; k++) candidate((float)w[k], at[u] + k);
+                    for (int k = 0; k < N; k++) take(o[k], at[u] + k);
                 }
         }
     }
     __syncthreads();
     int n = sh.n;
     if (!fits || n > Shared<JOIN_NT>::MAX_KEYS || n < a.top) {  // (the same for every thread)
-        n = a.top;
-        select_any<T, JOIN_NT>(x, Span<T>(x, a.V), n, order_of(tau), sh, tid);
+        n = select_any<T, JOIN_NT>(x, Span<T>(x, a.V), a.top, order_of(tau), sh, tid);
     }
     in_order<JOIN_NT>(sh.key, n, a.top, tid, [&](unsigned long long key, int k) {
         a.top_tokens[(int64_t)r * a.top + k] = index_of(key);

@@ -218,6 +218,31 @@ def test_logprobs_long_rows(rows, V, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V", [2500, 20003, 40000, 131075])
+def test_logprobs_rows_whose_threshold_is_low(V, dtype):
+    """Rows whose waves see very different elements, so that most of the row lies above the threshold that all of them agree
+    on; with masks, a NaN or few entries left besides."""
+    gen = torch.Generator().manual_seed(V)
+    x = (torch.randn((6, V), generator=gen) * 3.0).to(dtype)
+    width = 16 // x.element_size()
+    low = ((torch.arange(V) // width) % 256 < 64).expand(6, V).clone()  # a wave's elements of four
+    x = torch.where(low, x - 20, x)
+    x[1] = x[1].masked_fill(low[1], float("-inf"))
+    x[2] = x[2].masked_fill(low[2], torch.finfo(dtype).min)
+    x[3, V // 2] = float("nan")
+    few = torch.rand(V, generator=gen) < 8.0 / V
+    x[4] = x[4].masked_fill(~few, float("-inf"))
+    x[5] = x[5].masked_fill(~few, torch.finfo(dtype).min)
+    x[4:, V // 3] = 1.0
+    x = x.to(DEV)
+    tokens = torch.full((6,), V // 3).to(DEV)
+    for top in (1, 20, 64):
+        print("logprobs, low threshold, V=%d top=%d %s" % (V, top, dtype), flush=True)
+        run_logprobs(x, tokens, top, True, top == 20, gen)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("V", [5, 1500, 30001])
 def test_logprobs_masked_infinite_and_nan(V, dtype):
     """Rows of nothing but -inf, of nothing but the type's lowest value, with the lowest value as the mask, with +inf, with
