@@ -126,9 +126,9 @@ constexpr int SORT_U = 4;       // groups of 64 positions whose reads are on the
 // that the first has listed, or, where a wave has met more than its list holds (a common token), over all again.
 // The lanes that hold the same token are found by one ballot for each bit of the token; the last of them moves the token's
 // cursor on for all, so 64 positions cost the same whether they hold one token or 64.
-template <int NT>
+template <int NT, int LIST>
 struct OrderShared {
-    unsigned list[NT / 64][SORT_LIST];
+    unsigned list[NT / 64][LIST];
     int below[NT / 64], wave[NT / 64];
 };
 // All positions, each wave its share: from * 64 up to to * 64.  The next round's reads are ahead of what f stores, so that a
@@ -188,8 +188,8 @@ struct LookAtAll {
 // tokens; begin and place count from this workgroup's first, `before` are the tokens of the workgroups before it.
 // `look(f)` calls f(token, the lanes that hold a real one, the lanes' positions counted from the wave's first) for all that
 // the wave has to look at, in ascending position.
-template <int NT, typename Look, typename Count, typename Emit>
-__device__ __forceinline__ void order_own(int block, int block_bits, int own_bits, int ids, int *s_at, OrderShared<NT> &sh, Look look, Count count,
+template <int NT, int LIST, typename Look, typename Count, typename Emit>
+__device__ __forceinline__ void order_own(int block, int block_bits, int own_bits, int ids, int *s_at, OrderShared<NT, LIST> &sh, Look look, Count count,
                                           Emit emit) {
     constexpr int NW = NT / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -199,7 +199,7 @@ __device__ __forceinline__ void order_own(int block, int block_bits, int own_bit
     // appends the own tokens of a group to the wave's list (a ring)
     const auto append = [&](uint64_t w, unsigned long long own, int pos, int &listed) {
         if ((own >> lane) & 1)
-            sh.list[wave][(listed + __popcll(own & ((1ull << lane) - 1))) & (SORT_LIST - 1)] =
+            sh.list[wave][(listed + __popcll(own & ((1ull << lane) - 1))) & (LIST - 1)] =
                 (unsigned)(w >> block_bits) << 22 | (unsigned)pos;
         listed += __popcll(own);
     };
@@ -253,7 +253,7 @@ __device__ __forceinline__ void order_own(int block, int block_bits, int own_bit
     // `n` listed tokens, from the first-th on, to their places
     const auto place = [&](int first, int n) {
         const bool own = lane < n;
-        const unsigned e = sh.list[wave][(first + (own ? lane : 0)) & (SORT_LIST - 1)];
+        const unsigned e = sh.list[wave][(first + (own ? lane : 0)) & (LIST - 1)];
         const int id = (int)(e >> 22);
         unsigned long long same = __ballot(own);
         if (same & __ballot(id != __builtin_amdgcn_readfirstlane(id)))
@@ -272,7 +272,7 @@ __device__ __forceinline__ void order_own(int block, int block_bits, int own_bit
         __builtin_amdgcn_wave_barrier();
     };
     int placed = 0;
-    if (listed > SORT_LIST) {  // the list was overwritten: once more, placing 64 whenever there are
+    if (listed > LIST) {  // the list was overwritten: once more, placing 64 whenever there are
         listed = 0;
         look([&](uint64_t w, unsigned long long is, int pos) {
             const unsigned long long own = is & __ballot(((int)w & block_mask) == block);
@@ -294,12 +294,12 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
                                                                   int *__restrict__ counts, int *__restrict__ starts,
                                                                   int *__restrict__ order_pos, int *__restrict__ order_tok) {
     extern __shared__ int s_at[];  // [SORT_NW][ids]: occurrences, then cursors
-    __shared__ OrderShared<SORT_NT> sh;
+    __shared__ OrderShared<SORT_NT, SORT_LIST> sh;
     const int block = (int)blockIdx.x, block_mask = (1 << block_bits) - 1;
     const int ids = (int)((V - block + block_mask) >> block_bits);
     const LookAtAll<SORT_NT> look(tokens, padding_idx, N, V);
     int first = 0;
-    order_own<SORT_NT>(
+    order_own<SORT_NT, SORT_LIST>(
         block, block_bits, own_bits, ids, s_at, sh, look,
         [&](int id, int begin, int n, int before, int own) {
             first = before;
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(SORT_NT) void embedding_gather_kernel(const int *__
                                                                    int *__restrict__ count, int *__restrict__ counts, int *__restrict__ starts,
                                                                    int *__restrict__ order_pos, int *__restrict__ order_tok) {
     extern __shared__ int s_at[];  // [SORT_NW][ids]
-    __shared__ OrderShared<SORT_NT> sh;
+    __shared__ OrderShared<SORT_NT, SORT_LIST> sh;
     __shared__ int s_before[SORT_NW];
     const int block = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ids = (int)((V - block + OWNERS - 1) / OWNERS);
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(SORT_NT) void embedding_gather_kernel(const int *__
         }
     };
     int first = 0;
-    order_own<SORT_NT>(
+    order_own<SORT_NT, SORT_LIST>(
         block, 8, own_bits, ids, s_at, sh, look,
         [&](int id, int begin, int n, int, int own) {
             for (int w = 0; w < SORT_NW; w++) first += s_before[w];
@@ -455,20 +455,27 @@ __global__ __launch_bounds__(SORT_NT) void embedding_gather_kernel(const int *__
         });
 }
 
-// Few positions: order and sums in one launch.  A workgroup owns up to 256 tokens of the vocabulary (as above) and 128 bytes
-// of columns, orders the positions of its tokens in LDS and sums: eight lanes a token, its rows in ascending position; a
-// token met more than HEAVY times by all the groups of eight, each every 32nd occurrence, and their sums in order.  Rows of
+// Few positions: order and sums in one launch.  A workgroup owns up to 256 tokens of the vocabulary (as above) and 256 bytes
+// of columns, orders the positions of its tokens in LDS and sums: sixteen lanes a token, its rows in ascending position; a
+// token met more than HEAVY times by all the groups of sixteen, each every 32nd occurrence, and their sums in order.  Rows of
 // tokens that do not occur are zeroed.
-// Every workgroup looks at all positions, so this pays while these, times the tiles of columns, are few: 100 positions of
-// 40000 x 512 float16 take 11.9 us (in three launches 17.4 us), 8192 of 8000 x 128 bfloat16 13.0 us (17.0 us), but 5120 of
-// 40000 x 512 47 us (22.6 us).  The two launches saved are also 5 us of the host's time, which a small training step waits
-// for.  (Measured and dropped: this kernel's sums behind embedding_order_kernel, two launches: 40 us for those 5120.)
-constexpr int DIRECT_NT = 256, DIRECT_LANES = 8, DIRECT_GROUPS = DIRECT_NT / DIRECT_LANES;
-constexpr int DIRECT_TOKENS = 8192, HEAVY = 32;
-constexpr int64_t DIRECT_LOOKS = 16384, DIRECT_VOCAB = 1 << 18;
+//
+// What bounds it: every workgroup looks at all positions, so positions times tiles of columns; and that it writes the rows in
+// strips, so their bytes.  In one launch and in three, of float16, a fifth of the tokens the same one:
+//    100 of  40000 x  512   13.6   17.4 us        3000 of 40000 x 512   20.0   19.7 us       8192 of 1000 x  64   14.3   17.4 us
+//    100 of 200000 x  512   44.9   49.2 us        8192 of 40000 x 512   30.6   22.5 us       1000 of 1000 x 2048  24.7   16.0 us
+// and of 200000 x 333 float32, 266 MB, 112.9 and 82.1 us for 100.  Near the limit they are equal on the GPU, and the two
+// launches saved are some 8 us of the host's time, which a small training step waits for.
+// (Strips of 128 bytes by 256 threads: 23 and 42 us where this has 20 and 31; sixteen rows of a heavy token on their way
+// instead of eight: 32 instead of 27 us for 100 of 65000 x 1024, for want of registers; two launches, the sums behind
+// embedding_order_kernel: 40 us for 5120 of 40000 x 512.)
+constexpr int DIRECT_NT = 512, DIRECT_LANES = 16, DIRECT_GROUPS = DIRECT_NT / DIRECT_LANES;
+constexpr int DIRECT_TOKENS = 8192, HEAVY = 32, DIRECT_OWN = 256;
+constexpr int DIRECT_LIST = DIRECT_TOKENS / (DIRECT_NT / 64);  // all that a wave looks at: no second look (common tokens: 34 -> 28 us)
+constexpr int64_t DIRECT_LOOKS = 18432, DIRECT_TILES = 8, DIRECT_VOCAB = 1 << 18, DIRECT_BYTES = 1 << 27;
 inline int64_t direct_tiles(int es, int64_t D) { return (D * es + 16 * DIRECT_LANES - 1) / (16 * DIRECT_LANES); }
 inline bool direct_pays(int es, int64_t N, int64_t V, int64_t D) {
-    return D * es >= 16 && N <= DIRECT_TOKENS && V <= DIRECT_VOCAB && direct_tiles(es, D) <= DIRECT_LOOKS &&
+    return D * es >= 16 && N <= DIRECT_TOKENS && V <= DIRECT_VOCAB && V * D * es <= DIRECT_BYTES && direct_tiles(es, D) <= DIRECT_TILES &&
            N * direct_tiles(es, D) <= DIRECT_LOOKS;
 }
 template <typename T>
@@ -477,14 +484,14 @@ __global__ __launch_bounds__(DIRECT_NT) void embedding_direct_kernel(const T *__
                                                                      int64_t D, int block_bits, int own_bits) {
     constexpr int E = VocabElem<T>::N;
     struct Sort {
-        OrderShared<DIRECT_NT> order;
-        int at[DIRECT_NT / 64 * DIRECT_NT];
+        OrderShared<DIRECT_NT, DIRECT_LIST> order;
+        int at[DIRECT_NT / 64 * DIRECT_OWN];
     };
     __shared__ union {
         Sort sort;
         float sum[DIRECT_GROUPS][DIRECT_LANES * E];
     } sh;
-    __shared__ int s_begin[DIRECT_NT], s_count[DIRECT_NT], s_heavy[DIRECT_TOKENS / HEAVY], s_heavies;
+    __shared__ int s_begin[DIRECT_OWN], s_count[DIRECT_OWN], s_heavy[DIRECT_TOKENS / HEAVY], s_heavies;
     extern __shared__ unsigned short s_pos[];  // [N]
     const int tid = threadIdx.x, lane = tid % DIRECT_LANES, group = tid / DIRECT_LANES;
     const int block = (int)blockIdx.x, block_mask = (1 << block_bits) - 1;
@@ -492,7 +499,7 @@ __global__ __launch_bounds__(DIRECT_NT) void embedding_direct_kernel(const T *__
     if (tid == 0) s_heavies = 0;
     __syncthreads();
     const LookAtAll<DIRECT_NT> look(tokens, padding_idx, N, V);
-    order_own<DIRECT_NT>(
+    order_own<DIRECT_NT, DIRECT_LIST>(
         block, block_bits, own_bits, ids, sh.sort.at, sh.sort.order, look,
         [&](int id, int begin, int n, int, int) {
             if (id < 0) return;
@@ -713,7 +720,7 @@ int backward(const void *g, int64_t gstride, const int64_t *tokens, float scale,
     // 256 workgroups own the vocabulary, fewer a smaller one, more where they would own too much each
     int block_bits = 0, own_bits = 0;
     while (block_bits < 8 && ((int64_t)2 << block_bits) <= V) block_bits++;
-    while (((V - 1) >> block_bits) + 1 > (direct ? DIRECT_NT : MAX_OWN)) block_bits++;
+    while (((V - 1) >> block_bits) + 1 > (direct ? DIRECT_OWN : MAX_OWN)) block_bits++;
     while (((int64_t)1 << own_bits) < ((V - 1) >> block_bits) + 1) own_bits++;
     if (direct) {
         hipLaunchKernelGGL(embedding_direct_kernel<T>, dim3(1u << block_bits, (unsigned)direct_tiles((int)sizeof(T), D)), dim3(DIRECT_NT),
