@@ -1,5 +1,5 @@
 // What the operators on the two ends of the vocabulary share (vocab_logprobs.hip, vocab_embedding.hip): element types,
-// 16-byte accesses, wave reductions of 64-bit keys.
+// 16-byte accesses, maxima in single instructions.
 #pragma once
 
 #include "common.hip.h"
@@ -79,8 +79,6 @@ struct VocabElem {
     typedef ChunkMax<T> Max;
     typedef T vecT __attribute__((ext_vector_type(N)));
     typedef float vecF __attribute__((ext_vector_type(N)));
-    __device__ static __forceinline__ float widen(T x) { return (float)x; }
-    __device__ static __forceinline__ T narrow(float x) { return (T)x; }
     __device__ static __forceinline__ void unpack(const vec16 &v, float (&o)[N]) {
         const vecT t = __builtin_bit_cast(vecT, v);
 #pragma unroll

@@ -117,9 +117,27 @@ __device__ __forceinline__ void append_keys(Shared<NT> &sh, const float (&o)[N],
         }
 }
 
-// The q-th largest of a wave's values, which hold no NaN; equal ones are counted one by one.  (A wave that has fewer than q
-// values above -inf: -inf.)
-__device__ __forceinline__ float wave_nth_largest(float v, float largest, int q) {
+// The q-th largest of a wave's values, which hold no NaN, equal ones counted one by one (fewer than q above -inf: -inf): the
+// largest taken away again and again, or, where that are many times, bit by bit as far down as the type has bits.
+template <typename T, int G>
+__device__ __forceinline__ float nth_largest_bitwise(const float (&v)[G], int q) {
+    unsigned t = 0;
+    for (unsigned bit = 0x80000000u; bit >= VocabElem<T>::LOWEST_BIT; bit >>= 1) {
+        const float trial = (t | bit) > LOWEST_ORDER ? value_of_order(t | bit) : NEG_INF_F;
+        int have = 0;
+#pragma unroll
+        for (int g = 0; g < G; g++) have += __popcll(__ballot(v[g] >= trial));
+        if (have >= q) t |= bit;
+    }
+    if (!(t & 0x80000000u)) t |= VocabElem<T>::LOWEST_BIT - 1;  // (a negative value's order has ones below its last bit)
+    return t > LOWEST_ORDER ? value_of_order(t) : NEG_INF_F;
+}
+template <typename T>
+__device__ __forceinline__ float nth_largest(float v, float largest, int q) {
+    if (q > 8) {
+        const float one[1] = {v};
+        return nth_largest_bitwise<T, 1>(one, q);
+    }
     for (;;) {
         const int equal = __popcll(__ballot(v == largest));
         q -= equal > 0 ? equal : 1;
@@ -282,27 +300,27 @@ __device__ __forceinline__ Part scan_part(const T *x, int n, int top, bool keep,
     const float mine = max2_raw(mx.value(), edge);
     if (lanes != nullptr) lanes[tid] = mine;
     float m = wave_max_raw(mine), tau = m;
-    if (NW == 1 && top > 24) {
-        // one wave and a long list: the top-th largest element itself, bit by bit over the registers, as far down as the type
-        // has bits (the lanes' maxima would leave a good part of the row)
-        unsigned t = 0;
-        for (unsigned bit = 0x80000000u; bit >= VocabElem<T>::LOWEST_BIT; bit >>= 1) {
-            const float trial = (t | bit) > LOWEST_ORDER ? value_of_order(t | bit) : NEG_INF_F;
-            int have = __popcll(__ballot(edge >= trial && ei >= 0));
+    if (NW == 1 && MAXC <= FEW && top > 24) {
+        // one wave, a short row and a long list: the top-th largest element itself (maxima would leave a good part of the row)
+        float o[MAXC * N + 1];
+        o[MAXC * N] = edge;
 #pragma unroll
-            for (int i = 0; i < MAXC; i++) {
-                float o[N];
-                opaque(buf[i]);
-                VocabElem<T>::unpack(buf[i], o);
-                const bool in = tid + i * NT < sp.nvec;
+        for (int i = 0; i < MAXC; i++) {
+            float c[N];
+            VocabElem<T>::unpack(buf[i], c);
 #pragma unroll
-                for (int k = 0; k < N; k++) have += __popcll(__ballot(o[k] >= trial && in));
-            }
-            if (have >= top) t |= bit;
+            for (int k = 0; k < N; k++) o[i * N + k] = tid + i * NT < sp.nvec ? c[k] : NEG_INF_F;
         }
-        tau = t > LOWEST_ORDER ? value_of_order(t) : NEG_INF_F;
+        tau = nth_largest_bitwise<T>(o, top);
+    } else if (NW == 1 && top > 24) {
+        // two maxima a lane: twice as many as the longest list, so that their top-th largest leaves little besides
+        typename VocabElem<T>::Max half[2];
+#pragma unroll
+        for (int i = 0; i < MAXC; i++) half[i & 1].take(cm[i]);
+        const float o[2] = {max2_raw(half[0].value(), edge), half[1].value()};
+        tau = nth_largest_bitwise<T>(o, top);
     } else if (top > 0) {
-        tau = wave_nth_largest(mine, m, (top + NW - 1) / NW);
+        tau = nth_largest<T>(mine, m, (top + NW - 1) / NW);
     }
     if (lane == 0) {
         sh.max[wave] = m;
@@ -466,7 +484,12 @@ __device__ __forceinline__ void in_order(const unsigned long long *keys, int n, 
     }
 }
 
-// A workgroup per row.
+// A workgroup per row, the whole of it in registers, so that memory is read once.  What bounds it is that read where the rows are
+// many: 6400 rows of 40000 float16 with 20 alternatives and entropy, 512 MB, take 89 us, 5.8 TB/s (a read alone reaches 6.4);
+// 5120 rows, a third of them left out, without alternatives, 274 MB, take 51 us, 5.3 TB/s, where a backward is to come: then
+// the reads leave the rows in the memory-side cache (past it 46 us, but the backward 139 us instead of 94).  One row of 40000 takes 6 us: the
+// launch, then load, maxima, sums and alternatives one behind the other.  Short rows are bound by these steps of each
+// workgroup: 16000 rows of 8000 float16 with 20 alternatives 53 us, 4.8 TB/s (without 45 us), of 1000 with 5 15 us (9 us).
 template <typename T, int NT, int MAXC>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(MAXC >= 16 ? 4 : 1))) void logprobs_kernel(const T *__restrict__ logits, LogprobArgs a) {
     __shared__ Shared<NT> sh;
@@ -492,7 +515,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(MAXC >= 16 ?
 }
 
 // A row in several parts, where it is more than the registers of a workgroup hold.  Each part's workgroup leaves its sums and
-// the maximum of every lane's elements in the workspace: two words, then PART_NT floats ...
+// the maximum of every lane's elements in the workspace: two words, then PART_NT floats (64 rows of 250007 float32, 64 MB, in
+// 13 parts each: 12.4 us, 5.2 TB/s, 832 workgroups being little more than three a CU) ...
 constexpr int PART_NT = 256, PART_MAXC = 20;
 constexpr int PART_WORDS = 2 + PART_NT / 2;
 template <typename T>
@@ -517,10 +541,11 @@ __global__ __launch_bounds__(PART_NT) void logprobs_part_kernel(const T *__restr
 
 // ... and a workgroup per row joins the sums, rescaled to the row's maximum, and finds the alternatives: a threshold from the
 // lanes' maxima as scan_part takes it from its own, the lanes at or above it (hardly more than `top` of some thousand),
-// whose elements alone are read again, their candidates in order.  (Ordered lists from every part instead: 64 alternatives
-// of 64 rows of 250007 float32 in 38 us instead of 25 us.)
-constexpr int JOIN_NT = 1024;
-template <typename T>
+// whose elements alone are read again, their candidates in order.  It is a chain of three reads, each waiting for the one
+// before, 12.5 us of 1024 threads for 64 alternatives of 64 rows; where the rows are many, smaller workgroups that overlap
+// each other are faster (2000 rows of 131000 float16, both launches: 1024 threads 170 us, 256 126 us; 128 rows of 250007
+// float32: 35 and 38 us).  (Ordered lists from every part instead: 38 instead of 25 us for those 64 rows.)
+template <typename T, int JOIN_NT>
 __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restrict__ logits, LogprobArgs a, int part_len, int parts,
                                                                 const unsigned long long *__restrict__ work) {
     constexpr int N = VocabElem<T>::N, NW = JOIN_NT / 64, MAX_LANES = 512;
@@ -577,7 +602,7 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
 #pragma unroll
     for (int u = 0; u < U; u++) mine = max2_raw(mine, v[u]);
     for (int l0 = tid + U * JOIN_NT; l0 < all; l0 += JOIN_NT) mine = max2_raw(mine, lane_max(l0));
-    float tau = wave_nth_largest(mine, wave_max_raw(mine), (a.top + NW - 1) / NW);
+    float tau = nth_largest<T>(mine, wave_max_raw(mine), (a.top + NW - 1) / NW);
     if (lane == 0) sh.tau[wave] = tau;
     if (tid == 0) sh.n = s_lanes = 0;
     __syncthreads();
@@ -672,14 +697,20 @@ int launch_forward(const void *logits, const LogprobArgs &a, void *work, hipStre
         unsigned long long *w = (unsigned long long *)work;
         hipLaunchKernelGGL(logprobs_part_kernel<T>, row_grid(a.rows, c.parts), dim3(PART_NT), 0, s, x, a, c.len, w);
         PCFGNAT_HIP_CHECK(hipGetLastError());
-        hipLaunchKernelGGL(logprobs_join_kernel<T>, row_grid(a.rows), dim3(JOIN_NT), 0, s, x, a, c.len, c.parts, w);
+        if (a.rows < 192) hipLaunchKernelGGL((logprobs_join_kernel<T, 1024>), row_grid(a.rows), dim3(1024), 0, s, x, a, c.len, c.parts, w);
+        else hipLaunchKernelGGL((logprobs_join_kernel<T, 256>), row_grid(a.rows), dim3(256), 0, s, x, a, c.len, c.parts, w);
         PCFGNAT_HIP_CHECK(hipGetLastError());
         return PCFGNAT_OK;
     }
+    // The smallest workgroup whose registers hold the row without spilling: many small ones hide each other's latency, but where
+    // they do not fill the chip a row's own latency counts.  Of float16 with 5, 8 or 20 alternatives:
+    //    16000 rows of 8000, 20:  128 x 8 53 us, 256 x 4 67 us, 64 x 16 54 us         300 rows:  7.6, 6.5 and 9.0 us
+    //    6400 rows of 40000, 20:  256 x 20 89 us, 512 x 10 94 us, 1024 x 5 196 us     100 rows, 8:  7.5, 7.0 and 7.0 us
     // (every wave of a workgroup has to have elements: the alternatives' threshold is taken from all of them)
     if (chunks <= 64 * 2) launch_rows<T, 64, 2>(x, a, s);
     else if (chunks <= 64 * 8) launch_rows<T, 64, 8>(x, a, s);
-    else if (chunks <= 256 * 4) launch_rows<T, 256, 4>(x, a, s);
+    else if (chunks <= 256 * 4 && a.rows < 1024) launch_rows<T, 256, 4>(x, a, s);
+    else if (chunks <= 128 * 8) launch_rows<T, 128, 8>(x, a, s);
     else if (chunks <= 256 * 10) launch_rows<T, 256, 10>(x, a, s);
     else if (chunks <= 512 * 10 && a.rows < 512) launch_rows<T, 512, 10>(x, a, s);
     else if (chunks <= 256 * 20) launch_rows<T, 256, 20>(x, a, s);
@@ -695,7 +726,10 @@ struct LogprobGradArgs {
     int V, top;
 };
 
-// The gradient of one part of a row by one workgroup: NT threads, MAXC chunks of 16 bytes each, read once, written once.  The
+// The gradient of one part of a row by one workgroup: NT threads, MAXC chunks of 16 bytes each, read once, written once.  What bounds
+// it is memory: 5120 rows of 40000 float16, a third left out, 274 MB read and 410 MB written, take 90 us, 7.6 TB/s (part of the
+// reads comes from the memory-side cache, where the forward left them); 1001 rows of 50021 bfloat16 with four alternatives,
+// 190 MB in unaligned rows, 34 us, 5.6 TB/s.  Waves of 64 threads for rows of up to 128 chunks, otherwise 256.  The
 // chunks follow the alignment of the gradient's row; the logits' row may lie otherwise and is read unaligned.  The entries
 // at which something arrives besides (the token, the alternatives) are flagged by chunk in LDS, so that an ordinary chunk
 // pays one byte of LDS for them, and are added before the one rounding, in the order of the list.

@@ -201,7 +201,7 @@ def test_logprobs_contents(kind, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("rows,V", [(1, 40000), (2, 33333), (3, 131072), (300, 40000), (2, 262147)])
+@pytest.mark.parametrize("rows,V", [(1, 40000), (2, 33333), (3, 131072), (300, 40000), (2, 262147), (1100, 7001), (200, 90001)])
 def test_logprobs_long_rows(rows, V, dtype):
     gen = torch.Generator().manual_seed(rows + V)
     x = (torch.randn((rows, V), generator=gen) * 3.0).to(dtype).to(DEV)
