@@ -436,7 +436,7 @@ int pcfgnat_viterbi_decoding_host(const int64_t *pred_length, const int64_t *out
  * Log-probabilities of given tokens over rows of logits, with the entropy of each row and its top alternatives: one read of
  * the logits (no counterpart in the reference, whose model takes log_softmax and max,
  * glat_decomposed_with_link_two_hands_tri_pcfg.py:414-415; pcfgnat_logsoftmax_max is that).
- *   logits       outer x inner rows of V elements, F16 / BF16 / F32; row (b, p) starts at element
+ *   logits       outer x inner rows of V elements (at most 1,310,720), F16 / BF16 / F32; row (b, p) starts at element
  *                b * stride_outer + p * stride_inner, its elements are adjacent.  Any alignment of a whole element.
  *   tokens       int64 [outer, inner] contiguous, or NULL: log-probabilities are not asked for.
  *   logprobs     float32 [outer, inner]; NULL if and only if tokens is.
@@ -469,7 +469,8 @@ int pcfgnat_token_logprobs_backward(const void *logits, int dtype, int64_t outer
 /*
  * Embedding lookup with scaling: out[n] = scale * weight[tokens[n]], rounded once (what the decoder does with the glanced
  * tokens of nat_pcfg_loss.py:268 next).  weight [V, D], F16 / BF16 / F32, rows weight_stride elements apart; tokens int64
- * [N]; out [N, D] contiguous.  A negative token is a row of zeros, one at or beyond V a row of NaN.
+ * [N]; out [N, D] contiguous, not overlapping the weight.  N and V of up to 2^26, D of up to 2^20.  A negative token is a row
+ * of zeros, one at or beyond V a row of NaN.
  */
 int pcfgnat_token_embedding(const void *weight, int dtype, int64_t weight_stride, const int64_t *tokens, float scale,
                             void *out, int64_t N, int64_t V, int64_t D, void *stream);
@@ -478,7 +479,8 @@ int pcfgnat_token_embedding(const void *weight, int dtype, int64_t weight_stride
  * Its gradient: grad_weight[v] = scale * sum of grad_out[n] over the n with tokens[n] = v, in float32 in an order that
  * depends on the tokens alone (the same inputs give the same bits), rounded once; every row of grad_weight [V, D] (contiguous)
  * is written.  grad_out rows are grad_stride elements apart.  padding_idx (negative: none) and tokens outside [0, V) have no
- * gradient.  workspace: pcfgnat_token_embedding_backward_workspace_bytes bytes, 16-byte aligned.
+ * gradient.  workspace: pcfgnat_token_embedding_backward_workspace_bytes bytes, 16-byte aligned; may be NULL where that is 0.
+ * N of up to 2^26, V of up to 2^26, D of up to 2^20; grad_weight must not overlap grad_out.
  */
 size_t pcfgnat_token_embedding_backward_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D);
 int pcfgnat_token_embedding_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, float scale,
