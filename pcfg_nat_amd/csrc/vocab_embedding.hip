@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T *__restrict_
 // pieces of that order, joins of the sums of a token whose run was cut.  The order is a function of the tokens alone, so are the sums.
 //
 // What bounds it: writing all of dW (262 MB at 64000 x 2048 bfloat16, 38 us at the rate of a fill) and reading g once (32768
-// positions, 134 MB, 21 us); all launches of that case take 94 us, of 5120 positions of 40000 x 512 float16 22 us (41 and 5 MB, of
+// positions, 134 MB, 21 us); all launches of that case take 81 us, of 5120 positions of 40000 x 512 float16 22 us (41 and 5 MB, of
 // which 8 us the order).  A decoder input of a glanced graph holds one token in most places, so runs are cut evenly by
 // position, not by token.
 struct Plan {
@@ -576,7 +576,8 @@ __global__ __launch_bounds__(DIRECT_NT) void embedding_direct_kernel(const T *__
 // A wave sums one piece of the order over a tile of 64 chunks of columns, 8 rows of g on their way at a time.  Runs that begin
 // and end inside the piece are finished; the sums of the first and the last, where they go on outside, are left for the join.
 // The waves behind the last piece zero the rows that no token selects, beside the others' reads.  What bounds it is memory: 32768
-// positions of 64000 x 2048 bfloat16, 134 MB read and 262 MB written, take some 80 us, 4.9 TB/s (a copy reaches 5.05).
+// positions of 64000 x 2048 bfloat16, 134 MB read and 262 MB written, all launches 81 us, of which 14 the order and 7 the joins; with finished
+// rows that stay in the caches, too, 94 us (rows of zeros that stay there: 107 us; g read past them: 101 us).
 constexpr int SUM_U = 8;
 constexpr int ZERO_ROWS = 8;  // rows that one of them looks at
 template <typename T, bool NARROW>
@@ -647,7 +648,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const T *__restrict_
 #pragma unroll
                             for (int k = 0; k < E; k++) f[k] = acc[k] * scale;
                             if (NARROW) store_columns(dweight + (int64_t)tok * D, c, D, VocabElem<T>::pack(f));
-                            else *reinterpret_cast<vec16_any *>(dweight + (int64_t)tok * D + c) = VocabElem<T>::pack(f);
+                            else __builtin_nontemporal_store(VocabElem<T>::pack(f), reinterpret_cast<vec16_any *>(dweight + (int64_t)tok * D + c));
                         }
                     }
                     opened_before = false;
