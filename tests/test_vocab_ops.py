@@ -585,12 +585,13 @@ def _step(logits, tokens, weight, words, ups):
 
 
 def _step_inputs(seed, V, rows=37):
+    N = 300 if V < 10000 else 20000  # (the gradient of the embedding in one launch, in four)
     gen = torch.Generator().manual_seed(seed)
     logits = torch.randn((rows, V), generator=gen).half().to(DEV).requires_grad_(True)
     tokens = torch.randint(-1, V, (rows,), generator=gen).to(DEV)
     weight = torch.randn((500, 24), generator=gen).half().to(DEV).requires_grad_(True)
-    words = torch.where(torch.rand((300,), generator=gen) < 0.5, torch.tensor(3), torch.randint(0, 500, (300,), generator=gen)).to(DEV)
-    ups = [torch.randn(s, generator=gen).to(DEV) for s in ((rows,), (rows,), (rows, 3))] + [torch.randn((300, 24), generator=gen).half().to(DEV)]
+    words = torch.where(torch.rand((N,), generator=gen) < 0.5, torch.tensor(3), torch.randint(0, 500, (N,), generator=gen)).to(DEV)
+    ups = [torch.randn(s, generator=gen).to(DEV) for s in ((rows,), (rows,), (rows, 3))] + [torch.randn((N, 24), generator=gen).half().to(DEV)]
     return logits, tokens, weight, words, ups
 
 
