@@ -92,6 +92,25 @@ struct VocabElem {
     }
 };
 
+// Splits n elements at any element address into [head scalars][16-byte chunks][tail scalars].
+template <typename T>
+struct Span {
+    int head, nvec, tail;
+    __device__ __forceinline__ Span(const T *x, int n) {
+        constexpr int N = VocabElem<T>::N;
+        const int h = (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T));
+        head = h < n ? h : n;
+        nvec = (n - head) / N;
+        tail = n - head - nvec * N;
+    }
+    // the scalar of thread `tid` (one at most), or -1
+    __device__ __forceinline__ int edge(int tid) const {
+        if (tid < head) return tid;
+        if (tid < head + tail) return head + nvec * VocabElem<T>::N + (tid - head);
+        return -1;
+    }
+};
+
 inline int vocab_elem_bytes(int dtype) { return dtype == PCFGNAT_F32 ? 4 : 2; }
 inline bool vocab_dtype_ok(int dtype) { return dtype == PCFGNAT_F16 || dtype == PCFGNAT_BF16 || dtype == PCFGNAT_F32; }
 

@@ -470,7 +470,7 @@ __global__ __launch_bounds__(SORT_NT) void embedding_gather_kernel(const int *__
 // strips, so their bytes.  In one launch and in three, of float16, a fifth of the tokens the same one:
 //    100 of  40000 x  512   13.6   17.4 us        3000 of 40000 x 512   20.0   19.7 us       8192 of 1000 x  64   14.3   17.4 us
 //    100 of 200000 x  512   44.9   49.2 us        8192 of 40000 x 512   30.6   22.5 us       1000 of 1000 x 2048  24.7   16.0 us
-// and of 200000 x 333 float32, 266 MB, 112.9 and 82.1 us for 100.  Near the limit they are equal on the GPU, and the two
+// and of 200000 x 333 float32, 266 MB, 112.9 and 68.6 us for 100.  Near the limit they are equal on the GPU, and the two
 // launches saved are some 8 us of the host's time, which a small training step waits for.
 // (Strips of 128 bytes by 256 threads: 23 and 42 us where this has 20 and 31; sixteen rows of a heavy token on their way
 // instead of eight: 32 instead of 27 us for 100 of 65000 x 1024, for want of registers; two launches, the sums behind
@@ -575,14 +575,20 @@ __global__ __launch_bounds__(DIRECT_NT) void embedding_direct_kernel(const T *__
 
 // A wave sums one piece of the order over a tile of 64 chunks of columns, 8 rows of g on their way at a time.  Runs that begin
 // and end inside the piece are finished; the sums of the first and the last, where they go on outside, are left for the join.
-// The waves behind the last piece zero the rows that no token selects, beside the others' reads.  What bounds it is memory: 32768
+// The waves behind the last piece zero the rows that no token selects, beside the others' reads, neighbouring rows as one run in
+// aligned chunks (row by row: 100 positions of 200000 x 333 float32 81 us instead of 69, of 200000 x 64 float16 23 instead of 20).
+// What bounds it is memory: 32768
 // positions of 64000 x 2048 bfloat16, 134 MB read and 262 MB written, all launches 81 us, of which 14 the order and 7 the joins; with finished
 // rows that stay in the caches, too, 94 us (rows of zeros that stay there: 107 us; g read past them: 101 us).
 constexpr int SUM_U = 8;
-constexpr int ZERO_ROWS = 8;  // rows that one of them looks at
+inline int zero_rows_of(int64_t row_bytes) {  // rows that one of them looks at
+    int rows = 8;
+    while (rows < 64 && rows * row_bytes < 8192) rows *= 2;
+    return rows;
+}
 template <typename T, bool NARROW>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(const T *__restrict__ g, int64_t gstride, float scale, T *__restrict__ dweight,
-                                                            int64_t D, int tiles, int piece, int64_t pieces, int64_t V, const int *__restrict__ count,
+                                                            int64_t D, int tiles, int piece, int64_t pieces, int64_t V, int zero_rows, const int *__restrict__ count,
                                                             const int *__restrict__ counts, const int *__restrict__ order_pos,
                                                             const int *__restrict__ order_tok, float *__restrict__ cut) {
     constexpr int E = VocabElem<T>::N;
@@ -591,14 +597,17 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const T *__restrict_
     const int64_t p = task / tiles;
     if (p >= pieces) {
         const vec16 zero = {0u, 0u, 0u, 0u};
-        const int64_t v0 = (task - pieces * tiles) * ZERO_ROWS;
-        const bool unused = lane < ZERO_ROWS && v0 + lane < V && counts[v0 + lane < V ? v0 + lane : 0] == 0;
-        for (unsigned long long rows = __ballot(unused); rows; rows &= rows - 1) {
-            T *row = dweight + (v0 + __builtin_ctzll(rows)) * D;
-            if (NARROW) store_columns(row, 0, D, zero);
-            else
-                for (int64_t c = (int64_t)lane * E; c < D; c += 64 * E)
-                    __builtin_nontemporal_store(zero, reinterpret_cast<vec16_any *>(row + (c + E <= D ? c : D - E)));
+        const int64_t v0 = (task - pieces * tiles) * zero_rows;
+        unsigned long long rows = __ballot(lane < zero_rows && v0 + lane < V && counts[v0 + lane < V ? v0 + lane : 0] == 0);
+        while (rows) {  // runs of neighbouring rows
+            const int at = __builtin_ctzll(rows), n = ~(rows >> at) ? __builtin_ctzll(~(rows >> at)) : 64;
+            T *row = dweight + (v0 + at) * D;
+            const Span<T> sp(row, (int)(n * D));
+            const int e = sp.edge(lane);
+            if (e >= 0) row[e] = (T)0.f;
+            vec16 *to = reinterpret_cast<vec16 *>(row + sp.head);
+            for (int c = lane; c < sp.nvec; c += 64) __builtin_nontemporal_store(zero, to + c);
+            rows = n == 64 ? 0 : rows & ~(((1ull << n) - 1) << at);
         }
         return;
     }
@@ -740,7 +749,8 @@ int backward(const void *g, int64_t gstride, const int64_t *tokens, float scale,
     }
     const Plan p = plan_of(N, D);
     const int tiles = (int)((D + 64 * VocabElem<T>::N - 1) / (64 * VocabElem<T>::N));
-    const int64_t sum_blocks = (p.pieces * tiles + (V + ZERO_ROWS - 1) / ZERO_ROWS + 3) / 4;
+    const int zero_rows = zero_rows_of(D * (int64_t)sizeof(T));
+    const int64_t sum_blocks = (p.pieces * tiles + (V + zero_rows - 1) / zero_rows + 3) / 4;
     PCFGNAT_REQUIRE(sum_blocks <= MAX_BLOCKS, "token_embedding_backward: the gradient is too large for one call");
     char *w = (char *)workspace;
     int *count = (int *)w, *order_pos = (int *)(w + 16), *order_tok = (int *)(w + 16 + order_bytes(p));
@@ -767,10 +777,10 @@ int backward(const void *g, int64_t gstride, const int64_t *tokens, float scale,
     PCFGNAT_HIP_CHECK(hipGetLastError());
     if (D < VocabElem<T>::N)
         hipLaunchKernelGGL((embedding_sum_kernel<T, true>), dim3((unsigned)sum_blocks), dim3(256), 0, s, (const T *)g, gstride, scale,
-                           (T *)dweight, D, tiles, p.piece, p.pieces, V, count, counts, order_pos, order_tok, cut);
+                           (T *)dweight, D, tiles, p.piece, p.pieces, V, zero_rows, count, counts, order_pos, order_tok, cut);
     else
         hipLaunchKernelGGL((embedding_sum_kernel<T, false>), dim3((unsigned)sum_blocks), dim3(256), 0, s, (const T *)g, gstride, scale,
-                           (T *)dweight, D, tiles, p.piece, p.pieces, V, count, counts, order_pos, order_tok, cut);
+                           (T *)dweight, D, tiles, p.piece, p.pieces, V, zero_rows, count, counts, order_pos, order_tok, cut);
     PCFGNAT_HIP_CHECK(hipGetLastError());
     if (p.pieces > 1) {
         const unsigned split = (unsigned)((D + 255) / 256 < 64 ? (D + 255) / 256 : 64);

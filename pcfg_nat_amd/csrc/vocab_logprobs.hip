@@ -60,25 +60,6 @@ __device__ __forceinline__ const T *row_at(const T *logits, unsigned r, int64_t 
     return logits + (int64_t)b * so + (int64_t)(r - b * (unsigned)inner) * si;
 }
 
-// Splits n elements at any element address into [head scalars][16-byte chunks][tail scalars].
-template <typename T>
-struct Span {
-    int head, nvec, tail;
-    __device__ __forceinline__ Span(const T *x, int n) {
-        constexpr int N = VocabElem<T>::N;
-        const int h = (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T));
-        head = h < n ? h : n;
-        nvec = (n - head) / N;
-        tail = n - head - nvec * N;
-    }
-    // the scalar of thread `tid` (one at most), or -1
-    __device__ __forceinline__ int edge(int tid) const {
-        if (tid < head) return tid;
-        if (tid < head + tail) return head + nvec * VocabElem<T>::N + (tid - head);
-        return -1;
-    }
-};
-
 template <int NT>
 struct Shared {
     static constexpr int NW = NT / 64;
