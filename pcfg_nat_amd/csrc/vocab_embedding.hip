@@ -1,5 +1,5 @@
 // Scaled embedding lookup out[n] = scale * W[token_n] and its gradient dW[v] = scale * sum of g[n] over the n with
-// token_n = v, summed in float32 in ascending n and rounded once.  A negative token is a zero row, one at or beyond V a
+// token_n = v, summed in float32 in an order that the tokens alone decide, and rounded once.  A negative token is a zero row, one at or beyond V a
 // row of NaN; neither has a gradient, nor has the padding index.
 #include "vocab.hip.h"
 
