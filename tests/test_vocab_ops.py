@@ -267,6 +267,35 @@ def test_logprobs_masked_infinite_and_nan(V, dtype):
         run_logprobs(x.to(DEV), None, max(top, 1), True, False, gen)
 
 
+FAR = [s * m for m in (1.6e7, 1e8, 1e10, 1e20, 1e29) for s in (1, -1)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("far", FAR, ids="{:.1e}".format)
+def test_logprobs_far_from_zero(far, dtype):
+    """Rows whose largest entry, or whose mask, lies far from zero, where the product of the maximum and log2 e is rounded by more
+    than an exponent can hold: constant, one such entry among ordinary ones, a few ordinary ones among such, neighbouring values,
+    half of the row one behind the other (whole parts of a row that is cut), -inf besides.  In one part and in three."""
+    gen = torch.Generator().manual_seed(21)
+    for V in (9, 300, 20011, 90001 if dtype == torch.bfloat16 else 45007):
+        x = torch.randn((6, V), generator=gen) * 3.0
+        few = torch.rand((V,), generator=gen) < 5.0 / V
+        few[V // 2] = True
+        x[0] = far
+        x[1, V // 3] = far
+        x[2] = x[2].masked_fill(~few, far)
+        x[3] = far * (1.0 + torch.finfo(dtype).eps * torch.randint(0, 4, (V,), generator=gen))
+        x[4, :V // 2] = far
+        x[5] = far
+        x[5, ::2] = float("-inf")
+        x = x.to(dtype).to(DEV)
+        top = min(V, 7)
+        for tokens in (torch.full((6,), V // 3), torch.full((6,), V // 2), torch.tensor([0, 0, -1, V - 1, V - 1, V])):
+            print("logprobs far=%g V=%d %s" % (far, V, dtype), flush=True)
+            run_logprobs(x, tokens.to(DEV), top, True, True, gen)
+
+
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_logprobs_layouts(dtype):
