@@ -778,9 +778,10 @@ __global__ __launch_bounds__(NT) void logprobs_grad_kernel(const T *__restrict__
     float K = 0.f;
     for (int k = 0; k <= a.top; k++) K += s_g[k];
     K = __builtin_fmaf(gh, H, K);
+    // (below -200 the probability is 0 in float32; the bound keeps its product with gh, which may be large, from becoming 0 * inf)
     const auto of = [&](float v) {
         const float lp = (v - m) - lz;
-        return -__builtin_amdgcn_exp2f(lp * LOG2E) * __builtin_fmaf(gh, fmaxf(lp, -1e30f), K);
+        return -__builtin_amdgcn_exp2f(lp * LOG2E) * __builtin_fmaf(gh, fmaxf(lp, -200.f), K);
     };
     if (ei >= 0) {
         float g = of((float)edge);

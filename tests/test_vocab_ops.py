@@ -267,6 +267,21 @@ def test_logprobs_masked_infinite_and_nan(V, dtype):
         run_logprobs(x.to(DEV), None, max(top, 1), True, False, gen)
 
 
+def run_and_want_finite(logits, tokens, top, gen, arrives=None):
+    """As run_logprobs with its gradient, of rows without NaN and +inf: nothing of the results is NaN but where a token lies beyond
+    the vocabulary (a comparison with NaN holds nothing).  arrives: the gradient of every row's entropy, drawn otherwise."""
+    leaf = logits.detach().requires_grad_(True)
+    got = ops.token_logprobs(leaf, tokens, top=top, entropy=True)
+    ups = [torch.randn(t.shape, generator=gen).to(DEV) for t in got[:3]]
+    if arrives is not None:
+        ups[1] = torch.full_like(ups[1], arrives)
+    grad, = torch.autograd.grad(got[:3], leaf, ups)
+    known = tokens < logits.size(1)
+    assert not got.logprobs[known].isnan().any() and not got.entropy.isnan().any() and not got.top_logprobs.isnan().any()
+    assert grad[known].isfinite().all()
+    check_logprobs(logits, tokens, top, got, (grad, *ups))
+
+
 FAR = [s * m for m in (1.6e7, 1e8, 1e10, 1e20, 1e29) for s in (1, -1)]
 
 
@@ -293,7 +308,48 @@ def test_logprobs_far_from_zero(far, dtype):
         top = min(V, 7)
         for tokens in (torch.full((6,), V // 3), torch.full((6,), V // 2), torch.tensor([0, 0, -1, V - 1, V - 1, V])):
             print("logprobs far=%g V=%d %s" % (far, V, dtype), flush=True)
-            run_logprobs(x, tokens.to(DEV), top, True, True, gen)
+            run_and_want_finite(x, tokens.to(DEV), top, gen)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("arrives", [1e6, 1e9, -1e12], ids="{:.0e}".format)
+def test_logprobs_large_entropy_gradient(arrives, dtype):
+    """A gradient of the entropy as large as a scaled loss makes it: entries without probability (-inf, the lowest value, a large
+    negative number) have no gradient of their own, whatever arrives."""
+    gen = torch.Generator().manual_seed(22)
+    for V in (9, 300, 5000):
+        masks = [float("-inf"), torch.finfo(dtype).min, -1e30, -1e10, -300.0]
+        x = (torch.randn((len(masks), V), generator=gen) * 3.0).to(dtype)
+        for r, mask in enumerate(masks):
+            x[r, ::3] = mask
+        run_and_want_finite(x.to(DEV), torch.full((len(masks),), V // 2).to(DEV), 3, gen, arrives)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_finite_inputs_give_finite_results(dtype):
+    """No NaN out of numbers, masks and ordinary upstream gradients, over the ways in which both operators are launched."""
+    gen = torch.Generator().manual_seed(23)
+    for V in (1, 9, 300, 1001, 5000, 20011, 50021, 131075):
+        for kind in ("normal", "constant", "masked", "block", "large"):
+            x = content(kind, 5, V, gen).to(dtype)
+            if V > 2:
+                x[:, V - 1] = 0.5  # (an entry left in every row)
+            print("logprobs %s V=%d %s" % (kind, V, dtype), flush=True)
+            leaf = x.to(DEV).requires_grad_(True)
+            got = ops.token_logprobs(leaf, torch.full((5,), V - 1).to(DEV), top=min(V, 6), entropy=True)
+            ups = [torch.randn(t.shape, generator=gen).to(DEV) for t in got[:3]]
+            grad, = torch.autograd.grad(got[:3], leaf, ups)
+            # (a row of nothing but -inf, which a single masked entry is, has log-probabilities -inf)
+            assert not got.logprobs.isnan().any() and not got.top_logprobs.isnan().any()
+            assert got.entropy.isfinite().all() and grad.isfinite().all()
+    for V, N, D in ((1, 1, 1), (300, 100, 5), (300, 8192, 16), (5000, 3001, 333), (40000, 5120, 512), (70001, 20000, 40), (3, 33000, 8)):
+        weight = torch.randn((V, D), generator=gen).to(dtype).to(DEV).requires_grad_(True)
+        tokens = torch.where(torch.rand((N,), generator=gen) < 0.4, torch.tensor(0), torch.randint(-1, V, (N,), generator=gen)).to(DEV)
+        out = ops.token_embedding(weight, tokens, 2.0)
+        grad, = torch.autograd.grad(out, weight, torch.full_like(out, 0.125))  # (no sum leaves float16)
+        assert out.isfinite().all() and grad.isfinite().all(), (V, N, D)
 
 
 @gpu
