@@ -66,6 +66,12 @@ int pcfgnat_max_left3_viterbi_counts(unsigned long long *served, unsigned long l
 int pcfgnat_pipeline_redo_counts(unsigned long long *inside_sweeps, unsigned long long *viterbi_sentences,
                                  unsigned long long *inside_given_up, int reset);
 
+/* Diagnostic counter of pcfgnat_token_logprobs on the current device since the library was loaded (or the last reset): rows
+ * whose alternatives could not be taken from the elements above a threshold of the waves' maxima and were selected by reading
+ * the row again, up to some forty times.  It grows for rows of one value, with very many equal largest entries, with fewer
+ * entries left by a mask than alternatives asked for, or with a NaN; for ordinary rows it stays as it is. */
+int pcfgnat_token_logprobs_selections(unsigned long long *rows, int reset);
+
 #ifdef __cplusplus
 }
 #endif

@@ -82,6 +82,7 @@ SIGNATURES = {
     "pcfgnat_viterbi_decoding_host": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64]),
     "pcfgnat_token_logprobs_workspace_bytes": (ctypes.c_size_t, [_int, _i64, _i64, _int]),
     "pcfgnat_token_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "pcfgnat_token_logprobs_selections": (_int, [_vp, _int]),
     "pcfgnat_token_logprobs_backward": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "pcfgnat_token_embedding": (_int, [_vp, _int, _i64, _vp, ctypes.c_float, _vp, _i64, _i64, _i64, _vp]),
     "pcfgnat_token_embedding_backward_workspace_bytes": (ctypes.c_size_t, [_int, _i64, _i64, _i64]),

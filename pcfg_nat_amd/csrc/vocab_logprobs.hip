@@ -153,6 +153,8 @@ __device__ __forceinline__ void for_each(const T *x, const Span<T> &sp, int tid,
     }
 }
 
+__device__ unsigned long long g_selections;  // diagnostic: rows whose alternatives went through select_any
+
 // The `want` largest of a span whatever it holds (NaN, a constant, a mask that leaves fewer than `want`), where at least `want`
 // elements lie at or above `guess` in the order of `order_of`.  Everything above the guess is listed: where that is at least
 // `want` and fits (a NaN among ordinary logits) nothing else is done; where it is fewer (most of the span is one value, a
@@ -161,6 +163,7 @@ __device__ __forceinline__ void for_each(const T *x, const Span<T> &sp, int tid,
 template <typename T, int NT>
 __device__ __forceinline__ int select_any(const T *x, const Span<T> &sp, int want, unsigned guess, Shared<NT> &sh, int tid) {
     constexpr int N = VocabElem<T>::N;
+    if (tid == 0) atomicAdd(&g_selections, 1ULL);
     const vec16 *xv = reinterpret_cast<const vec16 *>(x + sp.head);
     const auto list_above = [&](unsigned t) {
         __syncthreads();
@@ -548,14 +551,18 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     const T *x = row_at(logits, r, a.inner, a.so, a.si, a.inner == a.rows);
     const T x_tok = x[tok < a.V ? tok : 0];
     const unsigned long long *in = work + (int64_t)r * parts * PART_WORDS;
-    // the lanes' maxima: U a thread on their way from here on, more than that are read again
-    constexpr int U = 4;
+    // the lanes' maxima: U a thread on their way from here on, more than that are read again.  Every wave takes the same
+    // number of lanes of every part, the threshold being taken from all waves: a wave without lanes (three parts have 768 for
+    // 1024 threads) or with those of one part alone, which may be masked, would send the row to select_any (64 rows of 50257
+    // float32, 20 alternatives: 196 us, as it is 12.8; 64 of 70001 with a quarter masked: 250 and 14).
+    constexpr int U = 4, SHARE = PART_NT / NW, AT_ONCE = 64 / SHARE;
     const int all = a.top > 0 ? parts * PART_NT : 0;
+    const auto lane_at = [&](int u) { return (lane / SHARE + u * AT_ONCE) * PART_NT + wave * SHARE + lane % SHARE; };
     const auto lane_max = [&](int l) { return reinterpret_cast<const float *>(in + (l / PART_NT) * PART_WORDS + 2)[l % PART_NT]; };
     float v[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int l = tid + u * JOIN_NT;
+        const int l = lane_at(u);
         v[u] = lane_max(l < all ? l : 0);  // (without alternatives nobody has written it and nobody looks at it)
         if (l >= all) v[u] = NEG_INF_F;
     }
@@ -586,7 +593,7 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     float mine = NEG_INF_F;
 #pragma unroll
     for (int u = 0; u < U; u++) mine = max2_raw(mine, v[u]);
-    for (int l0 = tid + U * JOIN_NT; l0 < all; l0 += JOIN_NT) mine = max2_raw(mine, lane_max(l0));
+    for (int u = U; lane_at(u) < all; u++) mine = max2_raw(mine, lane_max(lane_at(u)));
     float tau = nth_largest<T>(mine, wave_max_raw(mine), (a.top + NW - 1) / NW);
     if (lane == 0) sh.tau[wave] = tau;
     if (tid == 0) sh.n = s_lanes = 0;
@@ -601,8 +608,8 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restr
     };
 #pragma unroll
     for (int u = 0; u < U; u++)
-        if (tid + u * JOIN_NT < all) list(v[u], tid + u * JOIN_NT);
-    for (int l0 = tid + U * JOIN_NT; l0 < all; l0 += JOIN_NT) list(lane_max(l0), l0);
+        if (lane_at(u) < all) list(v[u], lane_at(u));
+    for (int u = U; lane_at(u) < all; u++) list(lane_max(lane_at(u)), lane_at(u));
     __syncthreads();
     const int lanes = s_lanes;
     bool fits = lanes <= MAX_LANES && z == z;
@@ -876,4 +883,15 @@ extern "C" int pcfgnat_token_logprobs_backward(const void *logits, int dtype, in
     if (dtype == PCFGNAT_F16) return launch_backward<f16>(logits, grad_logits, a, s);
     if (dtype == PCFGNAT_BF16) return launch_backward<bf16>(logits, grad_logits, a, s);
     return launch_backward<float>(logits, grad_logits, a, s);
+}
+
+extern "C" int pcfgnat_token_logprobs_selections(unsigned long long *rows, int reset) {
+    unsigned long long h = 0;
+    PCFGNAT_HIP_CHECK(hipMemcpyFromSymbol(&h, HIP_SYMBOL(g_selections), sizeof(h)));
+    if (rows) *rows = h;
+    if (reset) {
+        const unsigned long long z = 0;
+        PCFGNAT_HIP_CHECK(hipMemcpyToSymbol(HIP_SYMBOL(g_selections), &z, sizeof(z)));
+    }
+    return PCFGNAT_OK;
 }

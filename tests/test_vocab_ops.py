@@ -5,6 +5,8 @@ Tolerances.  u = 2^-24 is half a step of float32.  A sum of positive float32 ter
 a term) * u relative; a thread of the kernels adds at most 80 terms of its own, a few hundred partial sums follow where
 a row is split, and each exponential is off by less than (3 + |d|) u for its argument d.  200 u covers the sum with the terms
 that matter (|d| < 60).  Results in a narrower type are rounded once more, by half a step of that type."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -350,6 +352,47 @@ def test_finite_inputs_give_finite_results(dtype):
         out = ops.token_embedding(weight, tokens, 2.0)
         grad, = torch.autograd.grad(out, weight, torch.full_like(out, 0.125))  # (no sum leaves float16)
         assert out.isfinite().all() and grad.isfinite().all(), (V, N, D)
+
+
+def selections():
+    """Rows whose alternatives were selected by reading the row again, since the last call of this."""
+    torch.cuda.synchronize()
+    rows = ctypes.c_ulonglong()
+    _lib.check(_lib.load().pcfgnat_token_logprobs_selections(ctypes.byref(rows), 1), _lib.load())
+    return rows.value
+
+
+@gpu
+@pytest.mark.parametrize("dtype,V", [(torch.float16, 1000), (torch.float16, 8000), (torch.bfloat16, 40000), (torch.float32, 40000),
+                                     (torch.float16, 81921), (torch.bfloat16, 100277), (torch.float16, 122880), (torch.bfloat16, 131072),
+                                     (torch.float32, 40961), (torch.float32, 50257), (torch.float32, 61441), (torch.float32, 250007),
+                                     (torch.float32, 1310720)], ids=str)
+def test_logprobs_ordinary_rows_take_the_threshold(dtype, V):
+    """Alternatives of ordinary rows, in one part, in three and in more, of few rows and of many, come from the elements above the
+    threshold of the waves' maxima, also where a mask of -inf or of the lowest value covers all but one part of the row; those
+    of a constant row do not."""
+    gen = torch.Generator().manual_seed(V)
+    selections()
+    for rows in (1, 16, 191, 192):
+        x = (torch.randn((rows, V), generator=gen) * 3.0).to(dtype).to(DEV)
+        for top in (1, 20, 64):
+            print("logprobs V=%d rows=%d top=%d %s" % (V, rows, top, dtype), flush=True)
+            got = ops.token_logprobs(x, None, top=top, entropy=True)
+            assert selections() == 0, (rows, top)
+            if rows == 16 and top == 20:
+                check_logprobs(x[:2], None, top, [None] + [t[:2] for t in got[1:]])
+            if V < 40961:
+                continue
+            for low in (float("-inf"), torch.finfo(dtype).min):
+                for cut in (slice(0, V // 3 + 64), slice(V // 4, V)):
+                    y = x.clone()
+                    y[:, cut] = low
+                    got = ops.token_logprobs(y, None, top=top, entropy=True)
+                    assert selections() == 0, (rows, top, low, cut)
+                    if rows == 1 and top == 20:
+                        check_logprobs(y, None, top, got)
+        ops.token_logprobs(torch.full_like(x, 1.5), None, top=1)
+        assert selections() == rows  # (more equal elements than a workgroup puts in order: 256 for one wave, 1024 for more)
 
 
 @gpu
