@@ -91,12 +91,13 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T *__restrict_
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------
-// Three launches, no atomics on results: the positions in an order that groups them by token (ascending within it), sums over
-// pieces of that order, joins of the sums of a token whose run was cut.  The order is a function of the tokens alone, so are the sums.
+// No atomics on results.  Three launches: the positions in an order that groups them by token (ascending within it), sums over
+// pieces of that order, joins of the sums of a token whose run was cut.  Many positions take a fourth, for the order; few take
+// one launch for all.  The order is a function of the tokens alone, so are the sums.
 //
 // What bounds it: writing all of dW (262 MB at 64000 x 2048 bfloat16, 38 us at the rate of a fill) and reading g once (32768
-// positions, 134 MB, 21 us); all launches of that case take 81 us, of 5120 positions of 40000 x 512 float16 22 us (41 and 5 MB, of
-// which 8 us the order).  A decoder input of a glanced graph holds one token in most places, so runs are cut evenly by
+// positions, 134 MB, 21 us); the four launches of that case take 81 us, the three of 5120 positions of 40000 x 512 float16 20 to 24 us
+// (41 and 5 MB, of which 8 us the order).  A decoder input of a glanced graph holds one token in most places, so runs are cut evenly by
 // position, not by token.
 struct Plan {
     int64_t N;       // positions
@@ -126,8 +127,8 @@ constexpr int SORT_U = 4;       // groups of 64 positions whose reads are on the
 // sorted by frequency: in strips the first workgroup would place half of all tokens - and looks for them among all
 // positions, each wave in its sixteenth: first how often each occurs (and how many belong to the workgroups before this
 // one, which is where its part of the order begins: no workgroup waits for another), then each to its place, in ascending
-// position.  What bounds it is the look at every position, a dozen instructions for 64 (7.5 us for 5120 positions of 40000
-// tokens, 14 us for 32768 of 64000); the second look goes over the few
+// position.  What bounds it is the look at every position, a dozen instructions for 64 (8 us for 5120 positions of 40000
+// tokens, 11 us for 16384 of 64000, 77 us for 131072 of 300000); the second look goes over the few
 // that the first has listed, or, where a wave has met more than its list holds (a common token), over all again.
 // The lanes that hold the same token are found by one ballot for each bit of the token; the last of them moves the token's
 // cursor on for all, so 64 positions cost the same whether they hold one token or 64.
@@ -326,6 +327,9 @@ __global__ __launch_bounds__(SORT_NT) void embedding_order_kernel(const int64_t 
 // among the tokens of one owner by ballots within the wave, by counts over waves and owners in LDS.  Leaves the tile's tokens
 // and positions in that order and where each owner's begin (one more for the end) ...
 constexpr int SPREAD_NT = 512, SPREAD_Q = 4, SPREAD = SPREAD_NT * SPREAD_Q, OWNERS = 256;
+// The owners are OWNERS at most, each of MAX_OWN tokens: larger vocabularies keep the look at all positions, by more workgroups
+// still, which is a step in time from one row to the next (131072 positions of 262144 and of 262145 rows: 6.5 + 22 us and 77 us
+// for the order, 65 and 114 us a training pass at 16 columns; a million positions 249 and 682 us a pass).
 constexpr int SPREAD_FROM = 16384;  // positions
 __global__ __launch_bounds__(SPREAD_NT) void embedding_spread_kernel(const int64_t *__restrict__ tokens, int64_t padding_idx, int N, int64_t V,
                                                                      int *__restrict__ spread_tok, int *__restrict__ spread_pos,
@@ -469,11 +473,17 @@ __global__ __launch_bounds__(SORT_NT) void embedding_gather_kernel(const int *__
 // tokens that do not occur are zeroed.
 //
 // What bounds it: every workgroup looks at all positions, so positions times tiles of columns; and that it writes the rows in
-// strips, so their bytes.  In one launch and in three, of float16, a fifth of the tokens the same one:
-//    100 of  40000 x  512   13.6   17.4 us        3000 of 40000 x 512   20.0   19.7 us       8192 of 1000 x  64   14.3   17.4 us
-//    100 of 200000 x  512   44.9   49.2 us        8192 of 40000 x 512   30.6   22.5 us       1000 of 1000 x 2048  24.7   16.0 us
-// and of 200000 x 333 float32, 266 MB, 112.9 and 68.6 us for 100.  Near the limit they are equal on the GPU, and the two
-// launches saved are some 8 us of the host's time, which a small training step waits for.
+// strips, so their bytes.  In one launch and in three (replayed from a graph), of float16, a fifth of the tokens the same one:
+//    100 of  40000 x  512   13.6   17.4 us        3000 of 40000 x  512   19.6   19.3 us       8192 of  1000 x   64   14.3   17.4 us
+//   1000 of  40000 x 1024   22.7   24.4 us        4096 of 40000 x  512   22.0   20.1 us       8192 of 40000 x  512   30.6   22.5 us
+// At the limit of the looks, 18432, one launch takes up to 3.3 us more of the GPU and 6 to 7 us less of the host, whose 40 us a
+// small training step waits for (41 and 47 us a pass on either side of the limit):
+//   4600 of  40000 x  512   23.9   20.6 us        2300 of 40000 x 1024   28.0   25.0 us       6100 of 10007 x  384   19.3   18.8 us
+//   4700 of  40000 x  512   24.5   20.0 us        2400 of 40000 x 1024   28.4   25.4 us       6200 of 10007 x  384   20.7   18.9 us
+// The limit of the bytes, 2^27: below it one launch gains in all of these, above it some lose and others still gain.
+//    100 of 130000 x  512   23.7   33.0 us         100 of 132000 x 512   28.4   33.8 us        100 of 200000 x 512    37     49.4 us
+//   3000 of 130000 x  512   32.0   36.1 us        3000 of 132000 x 512   39.2   36.7 us
+//    100 of 100000 x  333 float32  28.1  36.6 us   100 of 101000 x 333 float32  28.5  37.2 us   100 of 200000 x 333 float32  102  69 us
 // (Strips of 128 bytes by 256 threads: 23 and 42 us where this has 20 and 31; sixteen rows of a heavy token on their way
 // instead of eight: 32 instead of 27 us for 100 of 65000 x 1024, for want of registers; two launches, the sums behind
 // embedding_order_kernel: 40 us for 5120 of 40000 x 512.)

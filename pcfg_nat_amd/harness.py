@@ -140,7 +140,9 @@ def decode_from_logits(logits, links, output_length, left_tree_mask, pad=PAD, be
     ``alternatives`` > 0: the same read of the logits also gives every graph node's that many most probable tokens and the
     entropy of its distribution (``ops.token_logprobs``, whose first alternative is the front-end's token), for confidences,
     rescoring or n-best lists; returns (tokens, pred_length, ``TokenLogprobs`` with ``entropy`` [B,L] and ``top_*``
-    [B,L,alternatives])."""
+    [B,L,alternatives]).  Every node has them, those behind ``output_length`` too.  The sweep then takes the first alternative's
+    log-probability, which differs from ``logsoftmax_max``'s in the last bits: where two trees score alike to within those,
+    the decode may choose another of them than without alternatives."""
     if alternatives > 0:
         nodes = ops.token_logprobs(logits, top=alternatives, entropy=True)
         tokens, pred_length = viterbi_decode(nodes.top_logprobs[..., 0].contiguous(), nodes.top_tokens[..., 0].contiguous(), links,

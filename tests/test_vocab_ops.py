@@ -2,9 +2,14 @@
 the formulas in float64, the conventions at the edges, layouts, and their refusals.
 
 Tolerances.  u = 2^-24 is half a step of float32.  A sum of positive float32 terms is off by at most (additions on the way of
-a term) * u relative; a thread of the kernels adds at most 80 terms of its own, a few hundred partial sums follow where
-a row is split, and each exponential is off by less than (3 + |d|) u for its argument d.  200 u covers the sum with the terms
-that matter (|d| < 60).  Results in a narrower type are rounded once more, by half a step of that type."""
+a term) * u relative.  A thread of the kernels adds at most 20 chunks of its own and one element besides, 81 terms of float32 and
+161 of the two-byte types; a wave's sum is 6 additions more, the waves' at most 8, the parts' of a row that is cut 6 and a
+factor: 178 u at most (98 u for float32).  An exponential is off by (3 + 2 |d|) u for its argument d (the instruction, the
+rounding of the argument and of log2 e), weighted by its share in the sum; the mean of |d| so weighted is H less log Z, at
+most 11 at 1310720 entries.  Together 203 u of Z (123 u for float32), of which the bounds' 220 u leave 17 for the logarithm and the
+subtractions, beside their 4 u of |d| and of |log Z|.  The entropy's own sum of exp(d) d is off by the same additions of its
+|log Z - H| and by 2 u of the mean of d squared, at most 130 u: less than 220 u (1 + |log Z - H|).  Results in a narrower type
+are rounded once more, by half a step of that type."""
 import ctypes
 
 import numpy as np
@@ -371,10 +376,10 @@ def test_logprobs_ordinary_rows_take_the_threshold(dtype, V):
     """Alternatives of ordinary rows, in one part, in three and in more, of few rows and of many, come from the elements above the
     threshold of the waves' maxima, also where a mask of -inf or of the lowest value covers all but one part of the row; those
     of a constant row do not."""
-    gen = torch.Generator().manual_seed(V)
+    gen = torch.Generator(device=DEV).manual_seed(V)
     selections()
     for rows in (1, 16, 191, 192):
-        x = (torch.randn((rows, V), generator=gen) * 3.0).to(dtype).to(DEV)
+        x = (torch.randn((rows, V), generator=gen, device=DEV) * 3.0).to(dtype)
         for top in (1, 20, 64):
             print("logprobs V=%d rows=%d top=%d %s" % (V, rows, top, dtype), flush=True)
             got = ops.token_logprobs(x, None, top=top, entropy=True)
