@@ -532,7 +532,8 @@ __global__ __launch_bounds__(PART_NT) void logprobs_part_kernel(const T *__restr
 // whose elements alone are read again, their candidates in order.  It is a chain of three reads, each waiting for the one
 // before, 11.4 us of 1024 threads for 64 alternatives of 64 rows; where the rows are many, smaller workgroups that overlap
 // each other are faster (both launches with 1024 and with 256 threads, 20 alternatives: 2000 rows of 131000 float16 162 and 116 us,
-// 256 rows of 250007 float32 53 and 52 us, 128 rows 31 and 33 us, 64 rows 20.5 and 23.4 us).  (Ordered lists from every part instead: 38 instead of 25 us for those 64 rows.)
+// 256 rows of 250007 float32 53 and 52 us, 128 rows 31 and 33 us, 64 rows 20.5 and 23.4 us).  (Ordered lists from every part
+// instead: 38 instead of 25 us for 64 alternatives of those 64 rows.)
 template <typename T, int JOIN_NT>
 __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const T *__restrict__ logits, LogprobArgs a, int part_len, int parts,
                                                                 const unsigned long long *__restrict__ work) {
